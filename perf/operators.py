@@ -8,7 +8,8 @@ operations, what a user writes without the library):
                                      holds element j low and j + 16 high; w = d * (q - 8))
   tree    q3_tree_attention          a tree of drafted tokens attends to the cache and to its own
                                      ancestors; its K/V rows go behind the cached ones
-  commit  q3_tree_commit             the accepted path's rows move together, in every layer
+  commit  q3_tree_commit             the accepted path's rows move together, in every layer; their
+                                     slots start with weight 0 and hold the path's positions
   scored  q3_decode_attention_scored one token's attention, which adds every slot's attention weight
                                      to an accumulator
   evict   q3_cache_evict             the slots with the largest accumulated weight and the newest
@@ -168,7 +169,7 @@ def prepare(case, seed):
         s["len"] = i64([max(0, S - T - (b * 13) % 64) for b in range(B)])
         s["new_len"] = torch.zeros(B, device="cuda", dtype=torch.int64)
         s["err"] = torch.zeros(1, device="cuda", dtype=torch.int32)
-    else:
+    if case["op"] != "tree":
         n = case.get("layers", 1)
         # weight a slot has drawn over some tens of steps: heavy tailed, largest for the first slots
         w = torch.exp(1.5 * randn(B, n, NKV, S)) * (32.0 / S)
@@ -178,6 +179,9 @@ def prepare(case, seed):
         gap = (torch.rand(B, n, NKV, S, generator=g, device="cuda") < 0.2).int()
         p = torch.arange(S, device="cuda", dtype=torch.int32) + gap.cumsum(-1, dtype=torch.int32)
         s["slot_pos"] = p
+        if case["op"] == "commit":
+            s["pos"] = s["len"] * 6 // 5
+            return s
         s["new_weight"] = torch.zeros_like(w)
         s["err"] = torch.zeros(1, device="cuda", dtype=torch.int32)
         if case["op"] == "evict":
@@ -270,7 +274,9 @@ def _plain_commit(s):
     k[b, :, :, dst] = k[b, :, :, src]
     v[b, :, :, dst] = v[b, :, :, src]
     s["new_len"].copy_(s["len"] + s["n"])
-    return {"k": s["k"], "v": s["v"], "len": s["new_len"]}
+    s["weight"][b, :, :, dst] = 0.0
+    s["slot_pos"][b, :, :, dst] = (s["pos"][b] + t).int()[:, None, None]
+    return {"k": s["k"], "v": s["v"], "weight": s["weight"], "slot_pos": s["slot_pos"], "len": s["new_len"]}
 
 
 def _plain_scored(s):
@@ -340,8 +346,9 @@ def _own(s):
         return {"out": s["out"], "k": s["k"], "v": s["v"]}
     if s["op"] == "commit":
         q3.call("q3_tree_commit", kv, 0, s["layers"], s["B"], s["A"], s["accepted"].data_ptr(), s["n"].data_ptr(),
-                s["len"].data_ptr(), s["new_len"].data_ptr(), s["err"].data_ptr(), st)
-        return {"k": s["k"], "v": s["v"], "len": s["new_len"]}
+                s["len"].data_ptr(), s["new_len"].data_ptr(), s["pos"].data_ptr(), s["weight"].data_ptr(),
+                s["slot_pos"].data_ptr(), s["err"].data_ptr(), st)
+        return {"k": s["k"], "v": s["v"], "weight": s["weight"], "slot_pos": s["slot_pos"], "len": s["new_len"]}
     if s["op"] == "scored":
         q3.call("q3_decode_attention_scored", s["qkv"].data_ptr(), s["q_norm"].data_ptr(), s["k_norm"].data_ptr(),
                 s["cos"].data_ptr(), s["sin"].data_ptr(), s["cos"].shape[0], kv, 0, s["B"], s["len"].data_ptr(),
@@ -381,8 +388,10 @@ def work(case):
         return {"bytes": b, "flops": sum(4 * HD * NQ * n * (c + (n + 1) / 2) for c, n in zip(lens, counts))}
     if op == "commit":
         A = case["A"]
-        moved = sum(A - (b * 2) % A - (b % 2 == 0) for b in range(case["B"])) * case["layers"] * NKV
-        return {"bytes": max(1, 2 * moved * row), "flops": 0}
+        heads = case["layers"] * NKV
+        kept = sum(A - (b * 2) % A for b in range(case["B"]))
+        stay = (case["B"] + 1) // 2  # paths that begin with the first token leave it where it is
+        return {"bytes": heads * (2 * (kept - stay) * row + 8 * kept), "flops": 0}
     # evict: the weights and positions in and out, and the rows of the kept slots behind the
     # budget, read and written (their number by chance: the newest, and their share of the rest)
     S, M, b = case["S"], case["budget"], 0.0
@@ -471,7 +480,9 @@ def exact(case, seed):
             for i, a in enumerate(s["accepted"][b].tolist()[:int(s["n"][b])]):
                 for x in (k, v):
                     x[b, :, :, m + i] = x[b, :, :, m + a].clone()
-        return {"k": s["k"], "v": s["v"], "len": s["len"] + s["n"]}
+                s["weight"][b, ..., m + i] = 0
+                s["slot_pos"][b, ..., m + i] = int(s["pos"][b]) + i
+        return {"k": s["k"], "v": s["v"], "weight": s["weight"], "slot_pos": s["slot_pos"], "len": s["len"] + s["n"]}
     M, w, sp = case["budget"], s["new_weight"], s["new_slot_pos"]
     for b, m in enumerate(lens):
         for l in range(case["layers"]):
