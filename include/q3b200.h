@@ -464,6 +464,108 @@ int q3_batch_trace_phases(q3_batch* m, int64_t steps, long long* out, int32_t* k
 int q3_batch_trace_kernels(q3_batch* m, int64_t steps, long long* out, int32_t* kinds,
                            int64_t cap, int64_t* n_kernels);
 
+/* ------------------------------------------------- drafted tokens, bounded cache
+ * Operators for speculative decoding and for caches that stay bounded: a
+ * 4-bit GEMV (a cheap draft of the Q8_0 projections), attention for a tree of
+ * drafted tokens, the move of an accepted path, one-token attention that
+ * accumulates attention weight per slot, and eviction by that weight.  None
+ * has a counterpart in the reference.  All enqueue on `stream` without
+ * allocating or synchronising, take no workspace, can be captured into
+ * graphs and run concurrently with one another on different buffers.
+ *
+ * Device-side checks: counts, lengths, positions and trees are DEVICE data.
+ * A sequence whose values are out of range is left as it was (its outputs and
+ * cache are not written) and a code goes into the device word *err if that is
+ * 0 (5: length, count or position; 6: tree or path); err may be NULL; read it
+ * with q3_check_error_word. */
+
+/* Q4_0 quantizer on host memory (n multiple of 32; out: n/32*18 bytes): blocks
+ * of 32 as GGUF holds them, [f16 d | 16 bytes], byte j with value j in its low
+ * nibble and value j+16 in its high one, value = d*(q - 8); d is the value of
+ * largest magnitude / -8, q the nearest of 0..15. */
+int q3_quantize_q4_0(const float* w, int64_t n, uint8_t* out);
+
+/* Q4_0 fused dequant + GEMV for R rows: y[R][N] = x[R][K] . W[N][K]^T, f32
+ * sums (tensor cores), f16 out, tolerance-level parity.  1 <= R <= 16, N >= 1,
+ * K multiple of 256, K <= 16384; w ([N][K/32] blocks) and x 16-byte aligned. */
+int q3_gemv_q4(const void* w, const void* x, void* y, int N, int K, int R, void* stream);
+
+/* A KV cache: f16 rows of 128, element (sequence b, layer l, slot s, kv head h)
+ * at b*seq_stride + l*layer_stride + s*slot_stride + h*head_stride (in f16
+ * elements, multiples of 8; strides of dimensions of size 1 are not used).
+ * Rows must not overlap.  The flat layout [B][layers*S][heads][128] and the
+ * head-major one [B][layers][heads][S][128] are both of this form.  q_heads /
+ * kv_heads is 1, 2, 4 or 8.  The struct is read during the call only. */
+typedef struct q3_kv_cache {
+  void* k;
+  void* v;
+  int64_t seq_stride, layer_stride, slot_stride, head_stride;
+  int64_t slots;  /* per layer */
+  int32_t layers;
+  int32_t q_heads, kv_heads;
+} q3_kv_cache;
+
+/* Attention of up to T drafted tokens per sequence, one layer.  Token i of
+ * sequence b has parent parents[b][i] (< i; -1: the last cached token), sits at
+ * RoPE position pos[b] + its number of ancestors, and attends to slots
+ * 0..len[b]-1, its ancestors and itself.  QK-RMSNorm + RoPE as in
+ * q3_decode_attention; the new K/V rows go to slots len[b] + i.
+ *   qkv:      f16 [B][T][(q_heads + 2 kv_heads) * 128] raw projections
+ *   n_tokens: DEVICE int32 [B], 0..T tokens (NULL: T each); rows behind them
+ *             are neither read nor written, a sequence with 0 is skipped
+ *   len, pos: DEVICE int64 [B]; len + n_tokens <= slots; after an eviction
+ *             len < pos
+ *   out:      f16 [B][T][q_heads * 128], 8-byte aligned like qkv
+ * 1 <= T <= 64 and T * q_heads / kv_heads <= 128.  rope tables f32
+ * [rope_rows, 64].  Tolerance-level parity; deterministic. */
+int q3_tree_attention(const void* qkv, const void* q_norm, const void* k_norm,
+                      const float* rope_cos, const float* rope_sin, int64_t rope_rows,
+                      const q3_kv_cache* cache, int layer, int B, int T, const int32_t* parents,
+                      const int32_t* n_tokens, const int64_t* len, const int64_t* pos, void* out,
+                      int* err, void* stream);
+
+/* After verification: the K/V rows of the accepted tokens accepted[b][0..n),
+ * n = n_accepted[b] (strictly ascending indices < 64 of drafted tokens), move
+ * from slots len[b] + accepted[b][i] to len[b] + i, in layers
+ * layer0..layer0+n_layers-1; new_len[b] = len[b] + n.  accepted: DEVICE int32
+ * [B][A], A <= 64; new_len lies apart from len.  A bad path moves nothing and
+ * gives new_len[b] = len[b].  Where the cache is evicted from (below), pos,
+ * weight and slot_pos are given (all three or none): the accepted slots start
+ * with weight 0 and hold positions pos[b] + i, the path's depths. */
+int q3_tree_commit(const q3_kv_cache* cache, int layer0, int n_layers, int B, int A,
+                   const int32_t* accepted, const int32_t* n_accepted, const int64_t* len,
+                   int64_t* new_len, const int64_t* pos, float* weight, int32_t* slot_pos,
+                   int* err, void* stream);
+
+/* One decode token per sequence, one layer: attention as q3_tree_attention with
+ * T = 1, and for each kv head new_weight[slot] = weight[slot] + the sum of the
+ * group's softmax weights for slots 0..len-1; slot len, the new token's, gets
+ * its own weight and slot_pos = pos.  Slots behind it are left as they were.
+ *   weight, new_weight: f32 [B][layers][kv_heads][slots], the same array or
+ *             apart; slot_pos: int32 of that shape, the position each slot holds
+ *   len:      -1 skips the sequence.
+ * slots up to 180,224 with two query heads per kv head (their scores stay on
+ * chip), in inverse proportion to that number. */
+int q3_decode_attention_scored(const void* qkv, const void* q_norm, const void* k_norm,
+                               const float* rope_cos, const float* rope_sin, int64_t rope_rows,
+                               const q3_kv_cache* cache, int layer, int B, const int64_t* len,
+                               const int64_t* pos, const float* weight, float* new_weight,
+                               int32_t* slot_pos, void* out, int* err, void* stream);
+
+/* Eviction down to `budget` slots, per (sequence, layer, kv head), in layers
+ * layer0..layer0+n_layers-1: where len[b] > budget, the slots kept are those
+ * with slot_pos >= pos[b] - recent, then those of the largest weight (a NaN
+ * counts least, ties go to the lower slot), budget in all.  Attention does not
+ * depend on slot order, so kept slots below the budget stay where they are, and
+ * those behind it move, in order, into the holes: K/V in place, weights and
+ * positions from weight / slot_pos to new_weight / new_slot_pos (apart from
+ * them).  new_len[b] = min(len[b], budget); nothing behind it is written.
+ * pos: the sequence's next position.  recent <= budget; slots <= 524288. */
+int q3_cache_evict(const q3_kv_cache* cache, int layer0, int n_layers, int B, int64_t budget,
+                   int64_t recent, const int64_t* len, const int64_t* pos, const float* weight,
+                   const int32_t* slot_pos, int64_t* new_len, float* new_weight,
+                   int32_t* new_slot_pos, int* err, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -298,6 +298,20 @@ static int ensure_smem_attr(F* fn, size_t bytes) {
   return Q3_OK;
 }
 
+// Clusters above 8 CTAs, likewise once for each kernel on each device.
+template <typename F>
+static int ensure_cluster_attr(F* fn) {
+  static std::set<std::pair<const void*, int>> done;
+  int dev = 0;
+  cudaGetDevice(&dev);
+  std::lock_guard<std::mutex> lk(g_attr_mu);
+  const auto key = std::make_pair((const void*)fn, dev);
+  if (done.count(key)) return Q3_OK;
+  Q3_CUDA(cudaFuncSetAttribute(fn, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+  done.insert(key);
+  return Q3_OK;
+}
+
 // Launch with optional programmatic dependent launch (PDL): the kernel may
 // begin while the previous kernel in the stream finishes; kernels call
 // griddepcontrol.wait before touching that kernel's outputs.
@@ -1998,3 +2012,11 @@ extern "C" int q3_model_trace_steps(q3_model* m, int64_t steps, int64_t trace_st
 #include "q3_batch.cuh"
 #include "q3_battn.cuh"
 #include "q3_batch_host.inc"
+
+// ---------------------------------------------------------------------------
+// drafted tokens over a bounded cache (4-bit GEMV, tree attention, eviction)
+// ---------------------------------------------------------------------------
+#include "q3_q4.cuh"
+#include "q3_tree.cuh"
+#include "q3_evict.cuh"
+#include "q3_cache_host.inc"

@@ -39,6 +39,7 @@ enum : int {
   kErrTimeoutGrid = 3,     // a grid barrier / flag wait gave up
   kErrBadToken = 4,        // token id outside the vocabulary
   kErrBadPos = 5,          // position outside the KV cache
+  kErrBadTree = 6,         // a parent that is no earlier token, an accepted path that does not ascend
 };
 
 // Spin budget for every wait in these kernels, in SM clock cycles (~1 s).

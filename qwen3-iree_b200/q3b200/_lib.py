@@ -30,9 +30,18 @@ class Weights(ctypes.Structure):
         "q8_ffn_down")]
 
 
+class KVCache(ctypes.Structure):
+    """struct q3_kv_cache -- device pointers, strides in f16 elements."""
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p),
+                *((n, ctypes.c_int64) for n in ("seq_stride", "layer_stride", "slot_stride",
+                                                "head_stride", "slots")),
+                *((n, ctypes.c_int32) for n in ("layers", "q_heads", "kv_heads"))]
+
+
 P, I, I64, U32, SZ = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_uint32, ctypes.c_size_t
 PP = ctypes.POINTER(ctypes.c_void_p)
 PI64 = ctypes.POINTER(ctypes.c_int64)
+PKV = ctypes.POINTER(KVCache)
 
 # name -> argtypes (all return int status unless listed in _RESTYPE)
 SIGNATURES = {
@@ -127,6 +136,12 @@ SIGNATURES = {
     "q3_batch_profile_steps": [P, I64, P, P, I64, PI64],
     "q3_batch_trace_phases": [P, I64, P, P, I64, PI64],
     "q3_batch_kernel_launches": [P, PI64],
+    "q3_quantize_q4_0": [P, I64, P],
+    "q3_gemv_q4": [P, P, P, I, I, I, P],
+    "q3_tree_attention": [P, P, P, P, P, I64, PKV, I, I, I, P, P, P, P, P, P, P],
+    "q3_tree_commit": [PKV, I, I, I, I, P, P, P, P, P, P, P, P, P],
+    "q3_decode_attention_scored": [P, P, P, P, P, I64, PKV, I, I, P, P, P, P, P, P, P, P],
+    "q3_cache_evict": [PKV, I, I, I, I64, I64, P, P, P, P, P, P, P, P, P],
     "q3_strerror": [I],
     "q3_last_error": [],
 }
