@@ -7,25 +7,33 @@
 //   out_i = sum_j softmax_j(q_i . k_j / sqrt(128)) v_j,   j over slots 0..m-1, i's ancestors and i.
 // The new K/V rows go to slots m + i.
 //
-// What it has to move is 512 bytes per (slot, kv head), once, for all 2 T query rows of that head, so
-// the work is split over the keys: a thread-block cluster of up to 16 CTAs owns a (sequence, kv head)
-// and each CTA a contiguous run of 64-key tiles, streamed by cp.async into a ring.  The softmax runs
-// online in registers; the CTAs' partial (max, sum, output) meet over distributed shared memory, so
-// there is no workspace, no counter and no second launch.
+// What it has to move is 512 bytes per (slot, kv head), once, for all group x T query rows of that
+// head, so the work is split over the keys: a thread-block cluster of up to 16 CTAs owns a (sequence,
+// kv head) and each CTA a contiguous run of 64-key tiles, streamed by cp.async into a ring of three
+// stages.  The softmax runs online; the CTAs' partial (max, sum, output) meet over distributed shared
+// memory, so there is no workspace, no counter and no second launch.
+//
+// Two kernels: up to 16 rows the products run as mma.sync, a warp taking 16 keys of each tile
+// (k_tree_attn); above that as tcgen05.mma on 128 rows, a thread taking one row (k_tree_tc).
 #pragma once
 
 #include "q3_attn.cuh"
 #include "q3_common.cuh"
 #include "q3_q4.cuh"
+#include "q3_tc.cuh"
 
 namespace q3 {
 
 constexpr int kTreeMaxTokens = 64;
 constexpr int kTreeThreads = 128;
-constexpr int kTreeTile = 64;                       // keys per ring stage
+constexpr int kTreeTile = 64;                             // keys per ring stage
 constexpr int kTreeStages = 3;
-constexpr int kTreeStageBytes = 2 * kTreeTile * kHD * 2;  // K then V
-constexpr int kTreeOPitch = kHD + 4;                // floats between partial output rows
+constexpr int kTreeHalf = kTreeTile * kHD * 2;            // a stage: K, then V
+constexpr int kTreeStageBytes = 2 * kTreeHalf;
+constexpr int kTreeOPitch = kHD + 4;                      // floats between partial output rows
+constexpr int kTreeSmallRows = 16;                        // rows of k_tree_attn
+constexpr int kTreeRows = 128;                            // rows of k_tree_tc
+constexpr float kTreeLog2Scale = kAttnScale * 1.44269504088896341f;  // scores in powers of two
 
 struct TreeArgs {
   const uint16_t* qkv;  // [B][T][(q_heads + 2 kv_heads) * 128]
@@ -81,331 +89,384 @@ __device__ __forceinline__ float4 ld_dsmem_f4(uint32_t local_addr, uint32_t rank
                : "memory");
   return v;
 }
+__device__ __forceinline__ void st_dsmem_u16(uint32_t local_addr, uint32_t rank, uint16_t v) {
+  asm volatile("st.shared::cluster.b16 [%0], %1;" ::"r"(dsmem_map(local_addr, rank)), "h"(v) : "memory");
+}
+__device__ __forceinline__ void st_dsmem_v2(uint32_t local_addr, uint32_t rank, uint2 v) {
+  asm volatile("st.shared::cluster.v2.b32 [%0], {%1, %2};" ::"r"(dsmem_map(local_addr, rank)), "r"(v.x),
+               "r"(v.y)
+               : "memory");
+}
 
-// Byte offset of 16-byte chunk c of row r in a tile of 256-byte rows: the low three chunk bits are
-// xored with the row, so that the 8 rows of an ldmatrix fall into different banks.
-__device__ __forceinline__ uint32_t tile_at(int r, int c) { return r * 256 + ((c ^ (r & 7)) << 4); }
+// Byte offset of 16-byte chunk c (0..15) of row r in a tile of ROWS 256-byte rows: two halves of 64
+// dims, each in the SWIZZLE_128B layout (128-byte rows, the chunk xored with the row).  The 8 rows of
+// an ldmatrix fall into different banks, and the tensor core reads it K-major (rows along N) or
+// MN-major (rows along K).
+template <int ROWS>
+__device__ __forceinline__ uint32_t tile_at(int r, int c) {
+  return (c >> 3) * (ROWS * 128) + r * 128 + (((c ^ r) & 7) << 4);
+}
 
-// One head vector through RMSNorm and RoPE by a warp into row `row` of a swizzled tile; returns this
-// lane's values (dims lane + 32 i).  The operations and roundings of norm_rope_vals.
-__device__ __forceinline__ void norm_rope_row(const float (&v)[4], const uint16_t (&gv)[4], float c0,
-                                              float s0, float c1, float s1, int lane, uint8_t* tile,
-                                              int row, uint16_t (&o)[4]) {
-  float ss = 0.0f;
+// What a CTA works on.
+struct TreeCta {
+  int C, rank, h, b, tid, warp, lane;
+  int n, R, nct, lo, tiles, fresh;  // tokens, rows, cached tiles; this CTA's first tile and tile count
+  int64_t len, pos;                 // fresh: 1 in the last CTA, whose tile 0 holds the new tokens
+  uint16_t *kb, *vb;
+  bool share;                       // the cluster's CTAs prepare the query rows for one another
+};
+
+// Reads and checks the sequence's values; false: nothing to do (the same in all CTAs of a cluster).
+template <bool SCORED>
+__device__ __forceinline__ bool tree_begin(const TreeArgs& a, TreeCta& c) {
+  c.C = gridDim.x, c.rank = blockIdx.x, c.h = blockIdx.y, c.b = blockIdx.z;
+  c.tid = threadIdx.x, c.warp = c.tid >> 5, c.lane = c.tid & 31;
+  c.n = SCORED ? 1 : (a.n_tokens ? a.n_tokens[c.b] : a.T);
+  c.len = a.len[c.b], c.pos = a.pos[c.b];
+  if (SCORED ? c.len == -1 : c.n == 0) return false;
+  if (c.n < 0 || c.n > a.T || c.len < 0 || c.len > a.S - c.n || c.pos < 0 || c.pos >= a.rope_rows) {
+    if (c.tid == 0 && a.err) atomicCAS(a.err, 0, kErrBadPos);
+    return false;
+  }
+  c.R = c.n << a.group_log2;
+  c.nct = (int)((c.len + kTreeTile - 1) / kTreeTile);
+  const int nt = c.nct + 1;  // the new tokens count as a last tile
+  c.lo = (int)((int64_t)c.rank * nt / c.C);
+  c.tiles = (int)((int64_t)(c.rank + 1) * nt / c.C) - c.lo;
+  c.fresh = c.rank == c.C - 1;
+  c.kb = a.k + c.b * a.seq_stride + c.h * a.head_stride;
+  c.vb = a.v + c.b * a.seq_stride + c.h * a.head_stride;
+  c.share = c.C > 1 && c.R > 8;
+  return true;
+}
+
+// Starts the copies of this CTA's tile j (not the new tokens') into its stage; rows behind the cached
+// slots are filled with zeros.
+__device__ __forceinline__ void tree_issue(const TreeArgs& a, const TreeCta& c, uint32_t ring, int j) {
+  const int64_t base = (int64_t)(c.lo + j - c.fresh) * kTreeTile;
+  const int r0 = c.tid >> 4, ch = c.tid & 15;
+  const uint32_t dst = ring + (j % kTreeStages) * kTreeStageBytes + tile_at<kTreeTile>(r0, ch);
+  const uint16_t* ks = c.kb + (base + r0) * a.slot_stride + ch * 8;
+  const uint16_t* vs = c.vb + (base + r0) * a.slot_stride + ch * 8;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) ss = __fmaf_rn(v[i], v[i], ss);
-  ss = warp_sum(ss);
-  const float r = __fsqrt_rn(__fadd_rn(__fdiv_rn(ss, 128.0f), kEps));
-  float n[4];
+  for (int k = 0; k < 8; ++k) {
+    const bool in = base + r0 + 8 * k < c.len;
+    cp_async16(dst + k * 1024, in ? ks : c.kb, in);
+    ks += 8 * a.slot_stride;
+  }
 #pragma unroll
-  for (int i = 0; i < 4; ++i) n[i] = h2f(f2h(__fmul_rn(__fdiv_rn(v[i], r), h2f(gv[i]))));
-  o[0] = f2h(__fsub_rn(__fmul_rn(n[0], c0), __fmul_rn(n[2], s0)));
-  o[2] = f2h(__fadd_rn(__fmul_rn(n[0], s0), __fmul_rn(n[2], c0)));
-  o[1] = f2h(__fsub_rn(__fmul_rn(n[1], c1), __fmul_rn(n[3], s1)));
-  o[3] = f2h(__fadd_rn(__fmul_rn(n[1], s1), __fmul_rn(n[3], c1)));
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int d = lane + 32 * i;
-    *reinterpret_cast<uint16_t*>(tile + tile_at(row, d >> 3) + (d & 7) * 2) = o[i];
+  for (int k = 0; k < 8; ++k) {
+    const bool in = base + r0 + 8 * k < c.len;
+    cp_async16(dst + kTreeHalf + k * 1024, in ? vs : c.vb, in);
+    vs += 8 * a.slot_stride;
   }
 }
 
-// Rows of q: r = token * group + j.  A warp owns MT * 16 of them and 64 / WK keys of a tile; WR warps
-// cover the rows, WK the keys (WR * WK = 4).
-template <int MT, int WR, int WK, bool SCORED>
-__global__ void __launch_bounds__(kTreeThreads, MT * WR * 16 <= 64 ? 2 : 1) k_tree_attn(const TreeArgs a) {
-  constexpr int RP = MT * WR * 16;       // rows, padded
-  constexpr int KW = kTreeTile / WK;     // keys of a tile per warp
-  constexpr int KS = KW < 32 ? KW : 32;  // keys per softmax step
-  extern __shared__ __align__(128) uint8_t smem[];
-  uint8_t* qs = smem;                                   // [RP][128] f16
-  uint8_t* ring = qs + RP * 256;                        // kTreeStages stages; then the partial outputs
-  float2* mlw = reinterpret_cast<float2*>(ring + kTreeStages * kTreeStageBytes);  // [WK][RP]
-  float2* ml = mlw + WK * RP;                           // [RP] this CTA's (max, sum)
-  unsigned long long* anc = reinterpret_cast<unsigned long long*>(ml + RP);  // [64] ancestors and self
-  int* up = reinterpret_cast<int*>(anc + kTreeMaxTokens);                    // [64]
-  float* score = reinterpret_cast<float*>(up + kTreeMaxTokens);              // [group][score_cap]
-  float* op = reinterpret_cast<float*>(ring);           // [WK][RP][kTreeOPitch]
+// Ancestors by doubling: after each step a token knows twice as many.  anc[i]: ancestors of i and i
+// itself; up: scratch.  false: a bad tree, or a token beyond the RoPE tables.
+__device__ __forceinline__ bool tree_ancestors(const TreeArgs& a, const TreeCta& c,
+                                               unsigned long long* anc, int* up) {
+  bool ok = true;
+  if (c.tid < c.n) {
+    const int p = a.parents[(int64_t)c.b * a.T + c.tid];
+    ok = p >= -1 && p < c.tid;
+    up[c.tid] = ok ? p : -1;
+    anc[c.tid] = 1ull << c.tid;
+  }
+  if (__syncthreads_or(!ok)) {
+    if (c.tid == 0 && a.err) atomicCAS(a.err, 0, kErrBadTree);
+    return false;
+  }
+  for (int s = 1; s < c.n; s <<= 1) {
+    unsigned long long m = 0;
+    int u = -1;
+    if (c.tid < c.n && up[c.tid] >= 0) m = anc[up[c.tid]], u = up[up[c.tid]];
+    __syncthreads();
+    if (c.tid < c.n) anc[c.tid] |= m, up[c.tid] = u;
+    __syncthreads();
+  }
+  if (__syncthreads_or(c.tid < c.n && c.pos + __popcll(anc[c.tid]) - 1 >= a.rope_rows)) {
+    if (c.tid == 0 && a.err) atomicCAS(a.err, 0, kErrBadPos);
+    return false;
+  }
+  return true;
+}
 
-  const int C = gridDim.x, rank = blockIdx.x, h = blockIdx.y, b = blockIdx.z;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-  const int wr = warp / WK, wk = warp % WK;
+// QK-RMSNorm and RoPE of the query rows into the tile `qs` (ROWS rows) of every CTA, and of the new K
+// rows, with the V rows as they are, into stage 0 of the last CTA and into the cache.  The operations
+// and roundings of norm_rope_vals, a warp per row, two rows at a time.  With `share` the rows are
+// dealt out to the cluster's CTAs, which push them to one another (the caller has waited until all
+// CTAs run, and follows with a cluster barrier); otherwise each CTA prepares all it needs.
+template <int ROWS, bool SCORED>
+__device__ __forceinline__ void tree_rows(const TreeArgs& a, const TreeCta& c,
+                                          const unsigned long long* anc, uint8_t* qs, uint8_t* ring) {
+  const int gl = a.group_log2, lane = c.lane;
+  const int64_t row_el = (int64_t)(a.q_heads + 2 * a.kv_heads) * kHD;
+  const uint16_t* qkv = a.qkv + (int64_t)c.b * a.T * row_el;
+  float gq[4], gk[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) gq[i] = h2f(a.q_norm[lane + 32 * i]), gk[i] = h2f(a.k_norm[lane + 32 * i]);
+  const int units = c.share || c.fresh ? c.R + c.n : c.R;
+  const int step = c.share ? 4 * c.C : 4;
+  const int last = c.C - 1;
+  for (int u0 = c.share ? c.rank + c.C * c.warp : c.warp; u0 < units; u0 += 2 * step) {
+    float v[2][4], cs[2][4];
+    uint2 vv[2];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int u = min(u0 + e * step, units - 1);  // a repeated row is computed and dropped
+      const bool isq = u < c.R;
+      const int tok = isq ? u >> gl : u - c.R;
+      const uint16_t* x = qkv + tok * row_el +
+                          (isq ? (c.h << gl) + (u & ((1 << gl) - 1)) : a.q_heads + c.h) * kHD;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[e][i] = h2f(x[lane + 32 * i]);
+      if (!isq) vv[e] = *reinterpret_cast<const uint2*>(x + a.kv_heads * kHD + lane * 4);
+      const int64_t p = (c.pos + (SCORED ? 0 : __popcll(anc[tok]) - 1)) * 64 + lane;
+      cs[e][0] = a.rope_cos[p], cs[e][1] = a.rope_cos[p + 32];
+      cs[e][2] = a.rope_sin[p], cs[e][3] = a.rope_sin[p + 32];
+    }
+    float ss[2] = {0.0f, 0.0f};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      ss[0] = __fmaf_rn(v[0][i], v[0][i], ss[0]);
+      ss[1] = __fmaf_rn(v[1][i], v[1][i], ss[1]);
+    }
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) {
+      const float y0 = __shfl_xor_sync(0xffffffffu, ss[0], off), y1 = __shfl_xor_sync(0xffffffffu, ss[1], off);
+      ss[0] = __fadd_rn(ss[0], y0), ss[1] = __fadd_rn(ss[1], y1);
+    }
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int u = u0 + e * step;
+      if (u >= units) break;
+      const bool isq = u < c.R;
+      const float r = __fsqrt_rn(__fadd_rn(__fdiv_rn(ss[e], 128.0f), kEps));
+      float x[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[i] = h2f(f2h(__fmul_rn(__fdiv_rn(v[e][i], r), isq ? gq[i] : gk[i])));
+      uint16_t o[4];
+      o[0] = f2h(__fsub_rn(__fmul_rn(x[0], cs[e][0]), __fmul_rn(x[2], cs[e][2])));
+      o[2] = f2h(__fadd_rn(__fmul_rn(x[0], cs[e][2]), __fmul_rn(x[2], cs[e][0])));
+      o[1] = f2h(__fsub_rn(__fmul_rn(x[1], cs[e][1]), __fmul_rn(x[3], cs[e][3])));
+      o[3] = f2h(__fadd_rn(__fmul_rn(x[1], cs[e][3]), __fmul_rn(x[3], cs[e][1])));
+      if (isq) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int d = lane + 32 * i;
+          *reinterpret_cast<uint16_t*>(qs + tile_at<ROWS>(u, d >> 3) + (d & 7) * 2) = o[i];
+        }
+        if (c.share) {  // half a warp a peer
+          __syncwarp();
+          const uint8_t* at = qs + tile_at<ROWS>(u, lane & 15);
+          const uint4 row = *reinterpret_cast<const uint4*>(at);
+          for (int p = lane >> 4; p < c.C; p += 2)
+            if (p != c.rank) st_dsmem_v4(smem_u32(at), p, row);
+        }
+      } else {
+        const int k = u - c.R;
+        uint16_t* kd = c.kb + (c.len + k) * a.slot_stride;
+        *reinterpret_cast<uint2*>(c.vb + (c.len + k) * a.slot_stride + lane * 4) = vv[e];
+        st_dsmem_v2(smem_u32(ring) + kTreeHalf + tile_at<kTreeTile>(k, lane >> 1) + (lane & 1) * 8, last, vv[e]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int d = lane + 32 * i;
+          kd[d] = o[i];
+          st_dsmem_u16(smem_u32(ring) + tile_at<kTreeTile>(k, d >> 3) + (d & 7) * 2, last, o[i]);
+        }
+      }
+    }
+  }
+  if (c.fresh)  // no weight falls on rows behind the new tokens, but 0 * NaN would
+    for (int r = c.n + c.warp; r < kTreeTile; r += 4)
+      *reinterpret_cast<uint2*>(ring + kTreeHalf + tile_at<kTreeTile>(r, lane >> 1) + (lane & 1) * 8) =
+          make_uint2(0u, 0u);
+}
+
+// Keys of tile j that row `row` sees, as bits; `nv`: keys the tile holds.
+__device__ __forceinline__ unsigned long long tree_seen(const TreeCta& c, const unsigned long long* anc,
+                                                        bool tree, int row, int nv, int gl) {
+  if (tree) return row < c.R ? anc[row >> gl] : 0ull;
+  return nv >= 64 ? ~0ull : (1ull << nv) - 1;
+}
+
+// This lane's factor for rank `lane`, and the row's max and sum over the cluster.
+__device__ __forceinline__ void tree_row_total(const TreeCta& c, const float2* ml, int r, float& M,
+                                               float& L, float& f) {
+  float2 q = make_float2(-INFINITY, 0.0f);
+  if (c.lane < c.C) {
+    q.x = ld_dsmem_f32(smem_u32(ml + r), c.lane);
+    q.y = ld_dsmem_f32(smem_u32(ml + r) + 4, c.lane);
+  }
+  M = warp_max(q.x);
+  f = ex2(__fsub_rn(q.x, M == -INFINITY ? 0.0f : M));
+  L = warp_sum(__fmul_rn(q.y, f));
+}
+
+// The cluster's partials (max and sum in ml, outputs in op) into the output: rank c takes rows c,
+// c + C, ..., a warp a row, four dims a lane.
+__device__ __forceinline__ void tree_output(const TreeArgs& a, const TreeCta& c, const float2* ml,
+                                            const float* op) {
   const int gl = a.group_log2, G = 1 << gl;
+  for (int r = c.rank + c.C * c.warp; r < c.R; r += c.C * 4) {
+    float M, L, f;
+    tree_row_total(c, ml, r, M, L, f);
+    float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
+    for (int k = 0; k < c.C; ++k) {
+      const float fk = __shfl_sync(0xffffffffu, f, k);
+      const float4 x = ld_dsmem_f4(smem_u32(op + r * kTreeOPitch + 4 * c.lane), k);
+      s.x = __fmaf_rn(x.x, fk, s.x), s.y = __fmaf_rn(x.y, fk, s.y);
+      s.z = __fmaf_rn(x.z, fk, s.z), s.w = __fmaf_rn(x.w, fk, s.w);
+    }
+    const float inv = L == 0.0f ? 0.0f : __fdiv_rn(1.0f, L);  // a row that sees nothing is zero
+    const uint2 w = make_uint2(pack_h2(__fmul_rn(s.x, inv), __fmul_rn(s.y, inv)),
+                               pack_h2(__fmul_rn(s.z, inv), __fmul_rn(s.w, inv)));
+    const int tok = r >> gl;
+    *reinterpret_cast<uint2*>(a.out + ((int64_t)c.b * a.T + tok) * a.q_heads * kHD +
+                              ((c.h << gl) + (r & (G - 1))) * kHD + c.lane * 4) = w;
+  }
+}
 
-  const int n = SCORED ? 1 : (a.n_tokens ? a.n_tokens[b] : a.T);
-  const int64_t len = a.len[b], pos = a.pos[b];
-  // every CTA of the cluster sees the same values and leaves together
-  if (SCORED ? len == -1 : n == 0) return;
-  bool bad = n < 0 || n > a.T || len < 0 || len > a.S - n || pos < 0 || pos >= a.rope_rows;
-  if (bad) {
-    if (tid == 0 && a.err) atomicCAS(a.err, 0, kErrBadPos);
+// Up to 16 query rows: r = token * group + j.  Each warp takes 16 keys of every tile, with a softmax
+// state of its own, so a tile costs it 16 + 16 MMAs and one pass over its K and V fragments.
+struct TreeSmallSmem {
+  static constexpr size_t bytes = kTreeStages * kTreeStageBytes + kTreeSmallRows * 256 +
+                                  5 * kTreeSmallRows * sizeof(float2) + kTreeMaxTokens * 12;
+};
+template <bool SCORED>
+__global__ void __launch_bounds__(kTreeThreads, 2) k_tree_attn(const TreeArgs a) {
+  constexpr int RP = kTreeSmallRows;
+  extern __shared__ __align__(128) uint8_t smem[];
+  uint8_t* ring = smem;                                                  // stages; then the partial outputs
+  uint8_t* qs = ring + kTreeStages * kTreeStageBytes;                    // [RP][128] f16
+  float2* mlw = reinterpret_cast<float2*>(qs + RP * 256);                // [4][RP] the warps' (max, sum)
+  float2* ml = mlw + 4 * RP;                                             // [RP] this CTA's
+  unsigned long long* anc = reinterpret_cast<unsigned long long*>(ml + RP);
+  int* up = reinterpret_cast<int*>(anc + kTreeMaxTokens);
+  float* score = reinterpret_cast<float*>(up + kTreeMaxTokens);          // [group][score_cap]
+  float* op = reinterpret_cast<float*>(ring);                            // [4][RP][kTreeOPitch]
+
+  TreeCta c;
+  if (!tree_begin<SCORED>(a, c)) return;
+  const int warp = c.warp, lane = c.lane, g = lane >> 2, t = lane & 3;
+  const int gl = a.group_log2, G = 1 << gl;
+  cluster_arrive();
+#pragma unroll
+  for (int j = 0; j < kTreeStages - 1; ++j) {
+    if (j >= c.fresh && j < c.tiles) tree_issue(a, c, smem_u32(ring), j);
+    cp_commit();
+  }
+  const bool ok = SCORED || tree_ancestors(a, c, anc, up);
+  cluster_wait();  // every CTA of the cluster runs
+  if (!ok) {
+    cp_wait<0>();
     return;
   }
-  const int R = n << gl;
-  const int nct = (int)((len + kTreeTile - 1) / kTreeTile), nt = nct + 1;  // the last tile: the new tokens
-  const int lo = (int)((int64_t)rank * nt / C), hi = (int)((int64_t)(rank + 1) * nt / C);
-  uint16_t* kb = a.k + b * a.seq_stride + h * a.head_stride;
-  uint16_t* vb = a.v + b * a.seq_stride + h * a.head_stride;
+  tree_rows<RP, SCORED>(a, c, anc, qs, ring);
+  if (c.share) cluster_sync_all();
+  else __syncthreads();
 
-  // cached tiles stream while the queries are prepared
-  auto issue_cached = [&](int i) {
-    const int64_t base = (int64_t)i * kTreeTile;
-    const int r0 = tid >> 4, c = tid & 15;
-    const uint32_t dst = smem_u32(ring) + ((i - lo) % kTreeStages) * kTreeStageBytes + tile_at(r0, c);
-    const uint16_t* ks = kb + (base + r0) * a.slot_stride + c * 8;
-    const uint16_t* vs = vb + (base + r0) * a.slot_stride + c * 8;
-#pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      const bool in = base + r0 + 8 * k < len;
-      cp_async16(dst + k * 2048, in ? ks : kb, in);
-      ks += 8 * a.slot_stride;
-    }
-#pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      const bool in = base + r0 + 8 * k < len;
-      cp_async16(dst + kTreeStageBytes / 2 + k * 2048, in ? vs : vb, in);
-      vs += 8 * a.slot_stride;
-    }
-  };
-#pragma unroll
-  for (int i = 0; i < kTreeStages - 1; ++i) {
-    if (lo + i < hi && lo + i < nct) issue_cached(lo + i);
-    cp_commit();
-  }
-
-  // ancestors by doubling: after step k a token knows 2^k of them
-  if (!SCORED) {
-    bool ok = true;
-    if (tid < n) {
-      const int p = a.parents[(int64_t)b * a.T + tid];
-      ok = p >= -1 && p < tid;
-      up[tid] = ok ? p : -1;
-      anc[tid] = 1ull << tid;
-    }
-    if (__syncthreads_or(!ok)) {
-      if (tid == 0 && a.err) atomicCAS(a.err, 0, kErrBadTree);
-      cp_wait<0>();
-      return;
-    }
-    for (int s = 1; s < n; s <<= 1) {
-      unsigned long long m = 0;
-      int u = -1;
-      if (tid < n && up[tid] >= 0) m = anc[up[tid]], u = up[up[tid]];
-      __syncthreads();
-      if (tid < n) anc[tid] |= m, up[tid] = u;
-      __syncthreads();
-    }
-    const bool far = tid < n && pos + __popcll(anc[tid]) - 1 >= a.rope_rows;
-    if (__syncthreads_or(far)) {
-      if (tid == 0 && a.err) atomicCAS(a.err, 0, kErrBadPos);
-      cp_wait<0>();
-      return;
-    }
-  }
-  const int row_el = (a.q_heads + 2 * a.kv_heads) * kHD;
-  const uint16_t* qkv = a.qkv + (int64_t)b * a.T * row_el;
-  auto rope_at = [&](int tok, float& c0, float& s0, float& c1, float& s1) {
-    const int64_t p = (pos + (SCORED ? 0 : __popcll(anc[tok]) - 1)) * 64;
-    c0 = a.rope_cos[p + lane], c1 = a.rope_cos[p + lane + 32];
-    s0 = a.rope_sin[p + lane], s1 = a.rope_sin[p + lane + 32];
-  };
-  {
-    uint16_t gq[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) gq[i] = a.q_norm[lane + 32 * i];
-#pragma unroll 2
-    for (int r = warp; r < RP; r += 4) {
-      if (r < R) {
-        const int tok = r >> gl;
-        const uint16_t* x = qkv + (int64_t)tok * row_el + ((h << gl) + (r & (G - 1))) * kHD;
-        float v[4], c0, s0, c1, s1;
-        uint16_t o[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = h2f(x[lane + 32 * i]);
-        rope_at(tok, c0, s0, c1, s1);
-        norm_rope_row(v, gq, c0, s0, c1, s1, lane, qs, r, o);
-      } else {
-        *reinterpret_cast<uint2*>(qs + r * 256 + lane * 8) = make_uint2(0u, 0u);
-      }
-    }
-  }
-  // the new tokens' tile: K rows normed and roped, V rows as they are, both also into the cache
-  auto issue_new = [&](int i) {
-    uint8_t* st = ring + ((i - lo) % kTreeStages) * kTreeStageBytes;
-    uint16_t gk[4];
-#pragma unroll
-    for (int i2 = 0; i2 < 4; ++i2) gk[i2] = a.k_norm[lane + 32 * i2];
-    const int np = (n + 31) & ~31;  // a step of up to 32 keys reads no further
-    for (int r = warp; r < np; r += 4) {
-      uint2* vd = reinterpret_cast<uint2*>(st + kTreeStageBytes / 2 + tile_at(r, lane >> 1) + (lane & 1) * 8);
-      if (r < n) {
-        const uint16_t* x = qkv + (int64_t)r * row_el + (a.q_heads + h) * kHD;
-        float v[4], c0, s0, c1, s1;
-        uint16_t o[4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) v[k] = h2f(x[lane + 32 * k]);
-        const uint2 vv = *reinterpret_cast<const uint2*>(x + a.kv_heads * kHD + lane * 4);
-        rope_at(r, c0, s0, c1, s1);
-        norm_rope_row(v, gk, c0, s0, c1, s1, lane, st, r, o);
-        uint16_t* kd = kb + (len + r) * a.slot_stride;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) kd[lane + 32 * k] = o[k];
-        *vd = vv;
-        *reinterpret_cast<uint2*>(vb + (len + r) * a.slot_stride + lane * 4) = vv;
-      } else {
-        *reinterpret_cast<uint2*>(st + r * 256 + lane * 8) = make_uint2(0u, 0u);
-        *vd = make_uint2(0u, 0u);
-      }
-    }
-  };
-#pragma unroll
-  for (int i = 0; i < kTreeStages - 1; ++i)
-    if (lo + i < hi && lo + i == nct) issue_new(nct);
-
-  constexpr float kC = kAttnScale * 1.44269504088896341f;  // scores in powers of two
-  float o[MT][16][4] = {}, m[MT][2], l[MT][2] = {};
-#pragma unroll
-  for (int i = 0; i < MT; ++i) m[i][0] = m[i][1] = -INFINITY;
+  float o[16][4] = {}, m[2] = {-INFINITY, -INFINITY}, l[2] = {};
   uint32_t qf[8][4];
-  const int qrow = wr * MT * 16 + (lane & 7) + ((lane >> 3) & 1) * 8;
-  if (MT == 1) {
-    __syncthreads();
 #pragma unroll
-    for (int kk = 0; kk < 8; ++kk) ldsm4(qf[kk], smem_u32(qs) + tile_at(qrow, 2 * kk + (lane >> 4)));
-  }
+  for (int kk = 0; kk < 8; ++kk)
+    ldsm4(qf[kk], smem_u32(qs) + tile_at<RP>((lane & 7) + ((lane >> 3) & 1) * 8, 2 * kk + (lane >> 4)));
 
-  for (int it = lo; it < hi; ++it) {
+  for (int j = 0; j < c.tiles; ++j) {
     cp_wait<kTreeStages - 2>();
     __syncthreads();
-    const int ahead = it + kTreeStages - 1;
-    if (ahead < hi) {
-      if (ahead < nct) issue_cached(ahead);
-      else issue_new(nct);
-    }
+    if (j + kTreeStages - 1 < c.tiles) tree_issue(a, c, smem_u32(ring), j + kTreeStages - 1);
     cp_commit();
-    const uint32_t st = smem_u32(ring) + ((it - lo) % kTreeStages) * kTreeStageBytes;
-    const bool fresh = it == nct;
-    const int nv = fresh ? n : (int)(len - (int64_t)it * kTreeTile < kTreeTile ? len - (int64_t)it * kTreeTile : kTreeTile);
-#pragma unroll 1
-    for (int k0 = wk * KW; k0 < wk * KW + KW && k0 < nv; k0 += KS) {
-      float s[MT][KS / 8][4] = {};
+    const uint32_t st = smem_u32(ring) + (j % kTreeStages) * kTreeStageBytes;
+    const bool fresh = j < c.fresh;
+    const int64_t left = c.len - (int64_t)(c.lo + j - c.fresh) * kTreeTile;
+    const int nv = fresh ? c.n : (int)(left < kTreeTile ? left : kTreeTile);
+    const int k0 = warp * 16;
+    if (k0 >= nv) continue;
+    float s[2][4] = {};
 #pragma unroll
-      for (int kk = 0; kk < 8; ++kk) {
-        uint32_t af[MT][4];
+    for (int kk = 0; kk < 8; ++kk) {
+      uint32_t bf[4];
+      ldsm4(bf, st + tile_at<kTreeTile>(k0 + (lane & 7) + (lane >> 4) * 8, 2 * kk + ((lane >> 3) & 1)));
+      mma_16816(s[0], qf[kk][0], qf[kk][1], qf[kk][2], qf[kk][3], bf[0], bf[1]);
+      mma_16816(s[1], qf[kk][0], qf[kk][1], qf[kk][2], qf[kk][3], bf[2], bf[3]);
+    }
+    if (fresh || nv < kTreeTile) {
 #pragma unroll
-        for (int i = 0; i < MT; ++i) {
-          if (MT == 1) {
+      for (int e = 0; e < 2; ++e) {
+        const unsigned long long see = tree_seen(c, anc, fresh && !SCORED, g + 8 * e, nv, gl);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) af[i][e] = qf[kk][e];
-          } else {
-            ldsm4(af[i], smem_u32(qs) + tile_at(qrow + 16 * i, 2 * kk + (lane >> 4)));
-          }
-        }
-#pragma unroll
-        for (int j = 0; j < KS / 16; ++j) {
-          uint32_t bf[4];
-          ldsm4(bf, st + tile_at(k0 + 16 * j + (lane & 7) + (lane >> 4) * 8, 2 * kk + ((lane >> 3) & 1)));
-#pragma unroll
-          for (int i = 0; i < MT; ++i) {
-            mma_16816(s[i][2 * j], af[i][0], af[i][1], af[i][2], af[i][3], bf[0], bf[1]);
-            mma_16816(s[i][2 * j + 1], af[i][0], af[i][1], af[i][2], af[i][3], bf[2], bf[3]);
-          }
-        }
+        for (int i = 0; i < 4; ++i)
+          if (!((see >> (k0 + 8 * (i >> 1) + 2 * t + (i & 1))) & 1)) s[i >> 1][2 * e + (i & 1)] = -INFINITY;
       }
-      if (fresh || nv < kTreeTile) {
+    }
+    if (SCORED && g < G) {
 #pragma unroll
-        for (int i = 0; i < MT; ++i)
+      for (int i = 0; i < 2; ++i)
+        *reinterpret_cast<float2*>(score + g * a.score_cap + j * kTreeTile + k0 + 8 * i + 2 * t) =
+            make_float2(s[i][0], s[i][1]);
+    }
+    uint32_t pf[2][2];
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const int row = wr * MT * 16 + 16 * i + g + 8 * e;
-            unsigned long long see = nv >= 64 ? ~0ull : (1ull << nv) - 1;
-            if (fresh && !SCORED) see = row < R ? anc[row >> gl] : 0ull;
+    for (int e = 0; e < 2; ++e) {
+      float mx = fmaxf(fmaxf(s[0][2 * e], s[0][2 * e + 1]), fmaxf(s[1][2 * e], s[1][2 * e + 1]));
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+      const float mn = fmaxf(m[e], __fmul_rn(mx, kTreeLog2Scale));
+      const float mu = mn == -INFINITY ? 0.0f : mn;  // a row that sees no key yet
+      const float al = ex2(__fsub_rn(m[e], mu));
+      m[e] = mn;
+      float sum = 0.0f;
 #pragma unroll
-            for (int j = 0; j < KS / 8; ++j)
-#pragma unroll
-              for (int c = 0; c < 2; ++c)
-                if (!((see >> (k0 + 8 * j + 2 * t + c)) & 1)) s[i][j][2 * e + c] = -INFINITY;
-          }
+      for (int i = 0; i < 2; ++i) {
+        const float p0 = ex2(__fmaf_rn(s[i][2 * e], kTreeLog2Scale, -mu));
+        const float p1 = ex2(__fmaf_rn(s[i][2 * e + 1], kTreeLog2Scale, -mu));
+        sum = __fadd_rn(sum, __fadd_rn(p0, p1));
+        pf[i][e] = pack_h2(p0, p1);
       }
-      if (SCORED && g < G) {
+      l[e] = __fmaf_rn(l[e], al, sum);
 #pragma unroll
-        for (int j = 0; j < KS / 8; ++j)
-          *reinterpret_cast<float2*>(score + g * a.score_cap + (it - lo) * kTreeTile + k0 + 8 * j + 2 * t) =
-              make_float2(s[0][j][0], s[0][j][1]);
+      for (int d = 0; d < 16; ++d) {
+        o[d][2 * e] = __fmul_rn(o[d][2 * e], al);
+        o[d][2 * e + 1] = __fmul_rn(o[d][2 * e + 1], al);
       }
-      uint32_t pf[MT][KS / 8][2];
+    }
 #pragma unroll
-      for (int i = 0; i < MT; ++i)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          float mx = -INFINITY;
-#pragma unroll
-          for (int j = 0; j < KS / 8; ++j) mx = fmaxf(mx, fmaxf(s[i][j][2 * e], s[i][j][2 * e + 1]));
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-          const float mn = fmaxf(m[i][e], __fmul_rn(mx, kC));
-          const float mu = mn == -INFINITY ? 0.0f : mn;  // a row that sees no key yet
-          const float al = ex2(__fsub_rn(m[i][e], mu));
-          m[i][e] = mn;
-          float sum = 0.0f;
-#pragma unroll
-          for (int j = 0; j < KS / 8; ++j) {
-            const float p0 = ex2(__fmaf_rn(s[i][j][2 * e], kC, -mu));
-            const float p1 = ex2(__fmaf_rn(s[i][j][2 * e + 1], kC, -mu));
-            sum = __fadd_rn(sum, __fadd_rn(p0, p1));
-            pf[i][j][e] = pack_h2(p0, p1);
-          }
-          l[i][e] = __fmaf_rn(l[i][e], al, sum);
-#pragma unroll
-          for (int d = 0; d < 16; ++d) {
-            o[i][d][2 * e] = __fmul_rn(o[i][d][2 * e], al);
-            o[i][d][2 * e + 1] = __fmul_rn(o[i][d][2 * e + 1], al);
-          }
-        }
-      const uint32_t sv = st + kTreeStageBytes / 2;
-#pragma unroll
-      for (int j = 0; j < KS / 16; ++j)
-#pragma unroll
-        for (int d = 0; d < 8; ++d) {
-          uint32_t bf[4];
-          ldsm4_t(bf, sv + tile_at(k0 + 16 * j + (lane & 7) + ((lane >> 3) & 1) * 8, 2 * d + (lane >> 4)));
-#pragma unroll
-          for (int i = 0; i < MT; ++i) {
-            mma_16816(o[i][2 * d], pf[i][2 * j][0], pf[i][2 * j][1], pf[i][2 * j + 1][0], pf[i][2 * j + 1][1],
-                      bf[0], bf[1]);
-            mma_16816(o[i][2 * d + 1], pf[i][2 * j][0], pf[i][2 * j][1], pf[i][2 * j + 1][0],
-                      pf[i][2 * j + 1][1], bf[2], bf[3]);
-          }
-        }
+    for (int d = 0; d < 8; ++d) {
+      uint32_t bf[4];
+      ldsm4_t(bf, st + kTreeHalf +
+                      tile_at<kTreeTile>(k0 + (lane & 7) + ((lane >> 3) & 1) * 8, 2 * d + (lane >> 4)));
+      mma_16816(o[2 * d], pf[0][0], pf[0][1], pf[1][0], pf[1][1], bf[0], bf[1]);
+      mma_16816(o[2 * d + 1], pf[0][0], pf[0][1], pf[1][0], pf[1][1], bf[2], bf[3]);
     }
   }
   cp_wait<0>();
   __syncthreads();  // the ring becomes the partial outputs
 
 #pragma unroll
-  for (int i = 0; i < MT; ++i)
+  for (int e = 0; e < 2; ++e) {
+    const int row = g + 8 * e;
+    float s = l[e];
+    s = __fadd_rn(s, __shfl_xor_sync(0xffffffffu, s, 1));
+    s = __fadd_rn(s, __shfl_xor_sync(0xffffffffu, s, 2));
+    if (t == 0) mlw[warp * RP + row] = make_float2(m[e], s);
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const int row = wr * MT * 16 + 16 * i + g + 8 * e;
-      float s = l[i][e];
-      s = __fadd_rn(s, __shfl_xor_sync(0xffffffffu, s, 1));
-      s = __fadd_rn(s, __shfl_xor_sync(0xffffffffu, s, 2));
-      if (t == 0) mlw[wk * RP + row] = make_float2(m[i][e], s);
-#pragma unroll
-      for (int d = 0; d < 16; ++d)
-        *reinterpret_cast<float2*>(op + (wk * RP + row) * kTreeOPitch + 8 * d + 2 * t) =
-            make_float2(o[i][d][2 * e], o[i][d][2 * e + 1]);
-    }
+    for (int d = 0; d < 16; ++d)
+      *reinterpret_cast<float2*>(op + (warp * RP + row) * kTreeOPitch + 8 * d + 2 * t) =
+          make_float2(o[d][2 * e], o[d][2 * e + 1]);
+  }
   __syncthreads();
-  // the key warps' partials into one per row: a warp a row, four dims a lane
-  for (int r = warp; r < R; r += 4) {
+  // the warps' partials into one per row: a warp a row, four dims a lane
+  for (int r = warp; r < c.R; r += 4) {
     float M = -INFINITY, L = 0.0f;
 #pragma unroll
-    for (int k = 0; k < WK; ++k) M = fmaxf(M, mlw[k * RP + r].x);
+    for (int k = 0; k < 4; ++k) M = fmaxf(M, mlw[k * RP + r].x);
     const float mu = M == -INFINITY ? 0.0f : M;
     float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
-    for (int k = 0; k < WK; ++k) {
+    for (int k = 0; k < 4; ++k) {
       const float2 q = mlw[k * RP + r];
       const float f = ex2(__fsub_rn(q.x, mu));
       const float4 x = *reinterpret_cast<const float4*>(op + (k * RP + r) * kTreeOPitch + 4 * lane);
@@ -413,40 +474,11 @@ __global__ void __launch_bounds__(kTreeThreads, MT * WR * 16 <= 64 ? 2 : 1) k_tr
       s.x = __fmaf_rn(x.x, f, s.x), s.y = __fmaf_rn(x.y, f, s.y);
       s.z = __fmaf_rn(x.z, f, s.z), s.w = __fmaf_rn(x.w, f, s.w);
     }
-    if (WK > 1) *reinterpret_cast<float4*>(op + r * kTreeOPitch + 4 * lane) = s;
+    *reinterpret_cast<float4*>(op + r * kTreeOPitch + 4 * lane) = s;
     if (lane == 0) ml[r] = make_float2(M, L);
   }
   cluster_sync_all();
-
-  // the cluster's partials into the output: rank c takes rows c, c + C, ...
-  auto row_total = [&](int r, float& M, float& L, float& f) {  // f: lane c's factor for rank c
-    float2 q = make_float2(-INFINITY, 0.0f);
-    if (lane < C) {
-      q.x = ld_dsmem_f32(smem_u32(ml + r), lane);
-      q.y = ld_dsmem_f32(smem_u32(ml + r) + 4, lane);
-    }
-    M = warp_max(q.x);
-    f = ex2(__fsub_rn(q.x, M == -INFINITY ? 0.0f : M));
-    L = warp_sum(__fmul_rn(q.y, f));
-  };
-  for (int r = rank + C * warp; r < R; r += C * 4) {
-    float M, L, f;
-    row_total(r, M, L, f);
-    float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 4
-    for (int c = 0; c < C; ++c) {
-      const float fc = __shfl_sync(0xffffffffu, f, c);
-      const float4 x = ld_dsmem_f4(smem_u32(op + r * kTreeOPitch + 4 * lane), c);
-      s.x = __fmaf_rn(x.x, fc, s.x), s.y = __fmaf_rn(x.y, fc, s.y);
-      s.z = __fmaf_rn(x.z, fc, s.z), s.w = __fmaf_rn(x.w, fc, s.w);
-    }
-    const float inv = L == 0.0f ? 0.0f : __fdiv_rn(1.0f, L);  // a row that sees nothing is zero
-    const uint2 w = make_uint2(pack_h2(__fmul_rn(s.x, inv), __fmul_rn(s.y, inv)),
-                               pack_h2(__fmul_rn(s.z, inv), __fmul_rn(s.w, inv)));
-    const int tok = r >> gl;
-    *reinterpret_cast<uint2*>(a.out + ((int64_t)b * a.T + tok) * a.q_heads * kHD +
-                              ((h << gl) + (r & (G - 1))) * kHD + lane * 4) = w;
-  }
+  tree_output(a, c, ml, op);
   if (SCORED) {
     // each slot's softmax weights of the group's heads join its accumulator, in f32
     float M[8], I[8];
@@ -454,30 +486,261 @@ __global__ void __launch_bounds__(kTreeThreads, MT * WR * 16 <= 64 ? 2 : 1) k_tr
     for (int j = 0; j < 8; ++j)
       if (j < G) {
         float L, f;
-        row_total(j, M[j], L, f);
+        tree_row_total(c, ml, j, M[j], L, f);
         if (M[j] == -INFINITY) M[j] = 0.0f;
         I[j] = L == 0.0f ? 0.0f : __fdiv_rn(1.0f, L);
       }
-    const int64_t w0 = b * a.w_stride + (int64_t)h * a.S, s0 = (int64_t)lo * kTreeTile;
-    const int64_t left = len - s0;
-    const int held = (int)(left < 0 ? 0 : left < (int64_t)(hi - lo) * kTreeTile ? left : (int64_t)(hi - lo) * kTreeTile);
-    for (int i = tid; i < held; i += kTreeThreads) {
+    const int64_t w0 = c.b * a.w_stride + (int64_t)c.h * a.S, s0 = (int64_t)c.lo * kTreeTile;
+    const int64_t span = (int64_t)(c.tiles - c.fresh) * kTreeTile, left = c.len - s0;
+    const int held = (int)(left < span ? left : span), first = c.fresh * kTreeTile;
+    for (int i = c.tid; i < held; i += kTreeThreads) {
       float w = a.w_in[w0 + s0 + i];
 #pragma unroll
       for (int j = 0; j < 8; ++j)
-        if (j < G) w = __fmaf_rn(ex2(__fmaf_rn(score[j * a.score_cap + i], kC, -M[j])), I[j], w);
+        if (j < G) w = __fmaf_rn(ex2(__fmaf_rn(score[j * a.score_cap + first + i], kTreeLog2Scale, -M[j])), I[j], w);
       a.w_out[w0 + s0 + i] = w;
     }
-    if (hi == nt && tid == 0) {  // the new slot starts with its own weight
+    if (c.fresh && c.tid == 0) {  // the new slot starts with its own weight
       float w = 0.0f;
 #pragma unroll
       for (int j = 0; j < 8; ++j)
-        if (j < G)
-          w = __fmaf_rn(ex2(__fmaf_rn(score[j * a.score_cap + (nct - lo) * kTreeTile], kC, -M[j])), I[j], w);
-      a.w_out[w0 + len] = w;
-      a.slot_pos[w0 + len] = (int32_t)pos;
+        if (j < G) w = __fmaf_rn(ex2(__fmaf_rn(score[j * a.score_cap], kTreeLog2Scale, -M[j])), I[j], w);
+      a.w_out[w0 + c.len] = w;
+      a.slot_pos[w0 + c.len] = (int32_t)c.pos;
     }
   }
+  cluster_sync_all();  // peers read this CTA's shared memory until here
+}
+
+// ---------------------------------------------------------------- above 16 rows: tcgen05
+// D[tmem] (+)= A[tmem] x B[smem desc], kind::f16 (f16 x f16 -> f32).
+__device__ __forceinline__ void umma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc,
+                                            uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// 32 consecutive columns of this thread's TMEM lane to / from registers.
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+        "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+        "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
+      "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+      "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]),
+      "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]),
+      "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// V as the B operand: rows are keys (the contraction), 64 dims a 128-byte row, MN-major.  8 keys are
+// 1024 bytes (the stride offset), the second 64 dims lie kTreeHalf / 2 behind (the leading offset).
+__device__ __forceinline__ uint64_t tree_v_desc(uint32_t saddr) {
+  uint64_t d = 0;
+  d |= (uint64_t)((saddr >> 4) & 0x3FFFu);
+  d |= (uint64_t)((kTreeHalf / 2) >> 4) << 16;
+  d |= (uint64_t)(1024u >> 4) << 32;
+  d |= (uint64_t)1u << 46;
+  d |= (uint64_t)2u << 61;
+  return d;
+}
+
+// TMEM columns: the queries (f16 pairs, the A operand of S = Q K^T), S (f32; its first half then holds
+// the weights as f16 pairs, the A operand of O += P V), and O.  256 in all: two CTAs an SM.
+constexpr uint32_t kTreeTmemCols = 256, kTreeTmemS = 64, kTreeTmemO = 128;
+
+struct TreeTcSmem {  // behind the ring
+  float2 ml[kTreeRows];
+  unsigned long long anc[kTreeMaxTokens];
+  int up[kTreeMaxTokens];
+  uint64_t s_done, o_done;
+  uint32_t tmem;
+};
+constexpr size_t kTreeTcBytes = 1024 + kTreeStages * kTreeStageBytes + sizeof(TreeTcSmem);
+
+// Thread r holds row r's softmax: one TMEM lane, no shuffles.  O stays in TMEM; it is rescaled only
+// when a row's maximum has grown by more than 2^8 since its last reference (the weights, relative to
+// that reference, stay below 2^8 and exact in form; sum and output share the reference).
+// Per tile: S = Q K^T (8 MMAs of 128 x 64 x 16), softmax, O += P V (4 of 128 x 128 x 16), one after the
+// other; the other CTA of the SM fills the gaps.
+__global__ void __launch_bounds__(kTreeThreads, 2) k_tree_tc(const TreeArgs a) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* ring = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  uint8_t* qs = ring + (kTreeStages - 1) * kTreeStageBytes;  // until the queries are in TMEM
+  TreeTcSmem& sm = *reinterpret_cast<TreeTcSmem*>(ring + kTreeStages * kTreeStageBytes);
+  float* op = reinterpret_cast<float*>(ring);                // [rows][kTreeOPitch], at the end
+
+  TreeCta c;
+  if (!tree_begin<false>(a, c)) return;
+  const int gl = a.group_log2, row = c.tid;
+  cluster_arrive();
+#pragma unroll
+  for (int j = 0; j < kTreeStages - 1; ++j) {
+    if (j >= c.fresh && j < c.tiles) tree_issue(a, c, smem_u32(ring), j);
+    cp_commit();
+  }
+  const bool tree_ok = tree_ancestors(a, c, sm.anc, sm.up);
+  cluster_wait();
+  if (!tree_ok) {
+    cp_wait<0>();
+    return;
+  }
+  if (c.tid == 0) {
+    mbar_init(&sm.s_done, 1);
+    mbar_init(&sm.o_done, 1);
+    fence_mbar_init();
+  }
+  if (c.warp == 0) {
+    tmem_alloc(&sm.tmem, kTreeTmemCols);
+    tmem_relinquish();
+  }
+  tree_rows<kTreeRows, false>(a, c, sm.anc, qs, ring);
+  asm volatile("fence.proxy.async;" ::: "memory");  // the new K and V rows, here or in the last CTA, go to MMAs
+  tc_fence_before();
+  if (c.share) cluster_sync_all();
+  else __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = sm.tmem, lane_base = tmem + ((uint32_t)(c.warp * 32) << 16);
+  const bool live = c.warp * 32 < c.R;  // warps of padding rows only copy and wait
+  if (live) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      uint32_t q[32];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const uint4 x = *reinterpret_cast<const uint4*>(qs + tile_at<kTreeRows>(row, 8 * i + k));
+        q[4 * k] = x.x, q[4 * k + 1] = x.y, q[4 * k + 2] = x.z, q[4 * k + 3] = x.w;
+      }
+      tmem_st32(lane_base + 32 * i, q);
+    }
+    tmem_wait_st();
+  }
+
+  constexpr uint32_t kIdS = idesc_f16_f32(128, kTreeTile);
+  constexpr uint32_t kIdO = idesc_f16_f32(128, kHD) | (1u << 16);  // B is MN-major
+  float m = -INFINITY, l = 0.0f;
+  bool ok = true;
+  int j = 0;
+  for (; j < c.tiles; ++j) {
+    cp_wait<kTreeStages - 2>();
+    fence_async_smem();
+    tc_fence_before();
+    __syncthreads();
+    const uint32_t st = smem_u32(ring) + (j % kTreeStages) * kTreeStageBytes;
+    if (c.tid == 0) {
+      tc_fence_after();
+      // P of the tile before shares columns with S
+      if (j > 0) ok &= mbar_wait_own(&sm.o_done, (j - 1) & 1, a.err, kErrTimeoutFull);
+      tc_fence_after();
+#pragma unroll
+      for (int kk = 0; kk < 8; ++kk)
+        umma_f16_ts(tmem + kTreeTmemS, tmem + 8 * kk, sw128_desc(st + (kk >> 2) * (kTreeHalf / 2) + (kk & 3) * 32),
+                    kIdS, kk != 0);
+      umma_commit(&sm.s_done);
+    }
+    ok &= mbar_wait_own(&sm.s_done, j & 1, a.err, kErrTimeoutFull);
+    tc_fence_after();
+    // the tile before is used up (its MMAs precede S): its stage takes the next copies
+    if (j + kTreeStages - 1 < c.tiles) tree_issue(a, c, smem_u32(ring), j + kTreeStages - 1);
+    cp_commit();
+    if (live) {
+      const bool fresh = j < c.fresh;
+      const int64_t left = c.len - (int64_t)(c.lo + j - c.fresh) * kTreeTile;
+      const int nv = fresh ? c.n : (int)(left < kTreeTile ? left : kTreeTile);
+      uint32_t u[64];
+      tmem_ld32(lane_base + kTreeTmemS, u);
+      tmem_ld32(lane_base + kTreeTmemS + 32, u + 32);
+      tmem_wait_ld();
+      if (fresh || nv < kTreeTile) {
+        const unsigned long long see = tree_seen(c, sm.anc, fresh, row, nv, gl);
+#pragma unroll
+        for (int i = 0; i < 64; ++i)
+          if (!((see >> i) & 1)) u[i] = 0xff800000u;
+      }
+      float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+      for (int i = 0; i < 64; ++i) mx[i & 3] = fmaxf(mx[i & 3], __uint_as_float(u[i]));
+      const float top = __fmul_rn(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])), kTreeLog2Scale);
+      const bool grow = top > __fadd_rn(m, 8.0f);  // from -inf: the first key that counts
+      const float mn = grow ? top : m;
+      const float mu = mn == -INFINITY ? 0.0f : mn;
+      if (j > 0 && __any_sync(0xffffffffu, grow)) {
+        const float al = grow ? ex2(__fsub_rn(m, mu)) : 1.0f;
+        l = __fmul_rn(l, al);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          uint32_t x[32];
+          tmem_ld32(lane_base + kTreeTmemO + 32 * i, x);
+          tmem_wait_ld();
+#pragma unroll
+          for (int k = 0; k < 32; ++k) x[k] = __float_as_uint(__fmul_rn(__uint_as_float(x[k]), al));
+          tmem_st32(lane_base + kTreeTmemO + 32 * i, x);
+        }
+      }
+      m = mn;
+      float sum[4] = {};
+      uint32_t p[32];
+#pragma unroll
+      for (int i = 0; i < 32; ++i) {
+        const float p0 = ex2(__fmaf_rn(__uint_as_float(u[2 * i]), kTreeLog2Scale, -mu));
+        const float p1 = ex2(__fmaf_rn(__uint_as_float(u[2 * i + 1]), kTreeLog2Scale, -mu));
+        sum[i & 3] = __fadd_rn(sum[i & 3], __fadd_rn(p0, p1));
+        p[i] = pack_h2(p0, p1);
+      }
+      l = __fadd_rn(l, __fadd_rn(__fadd_rn(sum[0], sum[1]), __fadd_rn(sum[2], sum[3])));
+      tmem_st32(lane_base + kTreeTmemS, p);
+      tmem_wait_st();
+    }
+    tc_fence_before();
+    if (__syncthreads_or(!ok)) break;
+    if (c.tid == 0) {
+      tc_fence_after();
+#pragma unroll
+      for (int ks = 0; ks < 4; ++ks)
+        umma_f16_ts(tmem + kTreeTmemO, tmem + kTreeTmemS + 8 * ks, tree_v_desc(st + kTreeHalf + 2048 * ks), kIdO,
+                    (j | ks) != 0);
+      umma_commit(&sm.o_done);
+    }
+  }
+  cp_wait<0>();
+  if (j > 0) mbar_wait_own(&sm.o_done, (j - 1) & 1, a.err, kErrTimeoutFull);
+  tc_fence_after();
+  __syncthreads();  // the ring becomes the partial outputs
+  if (live) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      uint32_t x[32];
+      tmem_ld32(lane_base + kTreeTmemO + 32 * i, x);
+      tmem_wait_ld();
+      if (row < c.R) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          *reinterpret_cast<uint4*>(op + row * kTreeOPitch + 32 * i + 4 * k) =
+              c.tiles > 0 ? make_uint4(x[4 * k], x[4 * k + 1], x[4 * k + 2], x[4 * k + 3]) : make_uint4(0, 0, 0, 0);
+      }
+    }
+    if (row < c.R) sm.ml[row] = make_float2(m, l);
+  }
+  tc_fence_before();
+  cluster_sync_all();
+  if (c.warp == 0) {
+    tc_fence_after();
+    tmem_dealloc(tmem, kTreeTmemCols);
+  }
+  tree_output(a, c, sm.ml, op);
   cluster_sync_all();  // peers read this CTA's shared memory until here
 }
 
