@@ -9,9 +9,11 @@
 //
 // What it has to move is 512 bytes per (slot, kv head), once, for all group x T query rows of that
 // head, so the work is split over the keys: a thread-block cluster of up to 16 CTAs owns a (sequence,
-// kv head) and each CTA a contiguous run of 64-key tiles, streamed by cp.async into a ring of three
-// stages.  The softmax runs online; the CTAs' partial (max, sum, output) meet over distributed shared
-// memory, so there is no workspace, no counter and no second launch.
+// kv head) and each CTA a contiguous run of 64-key tiles, streamed by tensor TMA into a ring.  (With
+// cp.async instead, 64 warp instructions a tile, the copies took 840 cycles of an SM a tile by
+// themselves, and 4800 when one warp issued them.)  The softmax runs online; the CTAs' partial (max,
+// sum, output) meet over distributed shared memory, so there is no workspace, no counter and no second
+// launch.
 //
 // Two kernels: up to 16 rows the products run as mma.sync, a warp taking 16 keys of each tile
 // (k_tree_attn); above that as tcgen05.mma on 128 rows, a thread taking one row (k_tree_tc).
@@ -25,17 +27,18 @@
 namespace q3 {
 
 constexpr int kTreeMaxTokens = 64;
-constexpr int kTreeThreads = 128;
+constexpr int kTreeThreads = 160;                         // four computing warps, a copying warp
 constexpr int kTreeTile = 64;                             // keys per ring stage
-constexpr int kTreeStages = 3;
 constexpr int kTreeHalf = kTreeTile * kHD * 2;            // a stage: K, then V
 constexpr int kTreeStageBytes = 2 * kTreeHalf;
 constexpr int kTreeOPitch = kHD + 4;                      // floats between partial output rows
+constexpr int kTreeMaxDepth = 6;                          // tiles a ring holds
 constexpr int kTreeSmallRows = 16;                        // rows of k_tree_attn
 constexpr int kTreeRows = 128;                            // rows of k_tree_tc
 constexpr float kTreeLog2Scale = kAttnScale * 1.44269504088896341f;  // scores in powers of two
 
 struct TreeArgs {
+  CUtensorMap km, vm;   // the layer's K and V: {dim, slot, head, sequence}, boxes of 64 dims x 64 slots
   const uint16_t* qkv;  // [B][T][(q_heads + 2 kv_heads) * 128]
   const uint16_t* q_norm;
   const uint16_t* k_norm;
@@ -140,26 +143,25 @@ __device__ __forceinline__ bool tree_begin(const TreeArgs& a, TreeCta& c) {
   return true;
 }
 
-// Starts the copies of this CTA's tile j (not the new tokens') into its stage; rows behind the cached
-// slots are filled with zeros.
-__device__ __forceinline__ void tree_issue(const TreeArgs& a, const TreeCta& c, uint32_t ring, int j) {
-  const int64_t base = (int64_t)(c.lo + j - c.fresh) * kTreeTile;
-  const int r0 = c.tid >> 4, ch = c.tid & 15;
-  const uint32_t dst = ring + (j % kTreeStages) * kTreeStageBytes + tile_at<kTreeTile>(r0, ch);
-  const uint16_t* ks = c.kb + (base + r0) * a.slot_stride + ch * 8;
-  const uint16_t* vs = c.vb + (base + r0) * a.slot_stride + ch * 8;
-#pragma unroll
-  for (int k = 0; k < 8; ++k) {
-    const bool in = base + r0 + 8 * k < c.len;
-    cp_async16(dst + k * 1024, in ? ks : c.kb, in);
-    ks += 8 * a.slot_stride;
-  }
-#pragma unroll
-  for (int k = 0; k < 8; ++k) {
-    const bool in = base + r0 + 8 * k < c.len;
-    cp_async16(dst + kTreeHalf + k * 1024, in ? vs : c.vb, in);
-    vs += 8 * a.slot_stride;
-  }
+// Cached keys of this CTA's tile j (at most 64 count).
+__device__ __forceinline__ int64_t tree_left(const TreeCta& c, int j) {
+  return c.len - (int64_t)(c.lo + j - c.fresh) * kTreeTile;
+}
+
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, int x, int y, int z,
+                                            int w, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes "
+      "[%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(smem_u32(bar))
+      : "memory");
+}
+// K or V of tile j (not the new tokens'), two boxes of 64 dims; slots behind the layer arrive as zeros.
+__device__ __forceinline__ void tree_copy(const TreeCta& c, const CUtensorMap* map, uint32_t dst, int j,
+                                          uint64_t* bar) {
+  const int slot = (c.lo + j - c.fresh) * kTreeTile;
+  tma_load_4d(dst, map, 0, slot, c.h, c.b, bar);
+  tma_load_4d(dst + kTreeHalf / 2, map, 64, slot, c.h, c.b, bar);
 }
 
 // Ancestors by doubling: after each step a token knows twice as many.  anc[i]: ancestors of i and i
@@ -278,10 +280,13 @@ __device__ __forceinline__ void tree_rows(const TreeArgs& a, const TreeCta& c,
       }
     }
   }
-  if (c.fresh)  // no weight falls on rows behind the new tokens, but 0 * NaN would
-    for (int r = c.n + c.warp; r < kTreeTile; r += 4)
-      *reinterpret_cast<uint2*>(ring + kTreeHalf + tile_at<kTreeTile>(r, lane >> 1) + (lane & 1) * 8) =
-          make_uint2(0u, 0u);
+}
+
+// V rows nv..63 of a tile become zeros, by a warp: no weight falls on rows behind the cached slots, or
+// behind the new tokens, but 0 * NaN would.
+__device__ __forceinline__ void tree_zero_tail(uint8_t* v, int nv, int lane) {
+  for (int i = nv * 16 + lane; i < kTreeTile * 16; i += 32)
+    *reinterpret_cast<uint4*>(v + tile_at<kTreeTile>(i >> 4, i & 15)) = make_uint4(0u, 0u, 0u, 0u);
 }
 
 // Keys of tile j that row `row` sees, as bits; `nv`: keys the tile holds.
@@ -331,60 +336,107 @@ __device__ __forceinline__ void tree_output(const TreeArgs& a, const TreeCta& c,
 
 // Up to 16 query rows: r = token * group + j.  Each warp takes 16 keys of every tile, with a softmax
 // state of its own, so a tile costs it 16 + 16 MMAs and one pass over its K and V fragments.
-struct TreeSmallSmem {
-  static constexpr size_t bytes = kTreeStages * kTreeStageBytes + kTreeSmallRows * 256 +
-                                  5 * kTreeSmallRows * sizeof(float2) + kTreeMaxTokens * 12;
+struct TreeSmallSmem {  // behind the ring
+  uint8_t q[kTreeSmallRows * 256];
+  float2 mlw[4][kTreeSmallRows];  // the warps' (max, sum)
+  float2 ml[kTreeSmallRows];      // this CTA's
+  unsigned long long anc[kTreeMaxTokens];
+  int up[kTreeMaxTokens];
+  uint64_t full[kTreeMaxDepth], empty[kTreeMaxDepth], tail;
 };
+constexpr size_t tree_small_bytes(int depth) {
+  return 1024 + (size_t)depth * kTreeStageBytes + sizeof(TreeSmallSmem);
+}
 template <bool SCORED>
-__global__ void __launch_bounds__(kTreeThreads, 2) k_tree_attn(const TreeArgs a) {
+__global__ void __launch_bounds__(kTreeThreads, 3)
+    k_tree_attn(const __grid_constant__ TreeArgs a, const int depth) {
   constexpr int RP = kTreeSmallRows;
   extern __shared__ __align__(128) uint8_t smem[];
-  uint8_t* ring = smem;                                                  // stages; then the partial outputs
-  uint8_t* qs = ring + kTreeStages * kTreeStageBytes;                    // [RP][128] f16
-  float2* mlw = reinterpret_cast<float2*>(qs + RP * 256);                // [4][RP] the warps' (max, sum)
-  float2* ml = mlw + 4 * RP;                                             // [RP] this CTA's
-  unsigned long long* anc = reinterpret_cast<unsigned long long*>(ml + RP);
-  int* up = reinterpret_cast<int*>(anc + kTreeMaxTokens);
-  float* score = reinterpret_cast<float*>(up + kTreeMaxTokens);          // [group][score_cap]
-  float* op = reinterpret_cast<float*>(ring);                            // [4][RP][kTreeOPitch]
+  uint8_t* ring = smem + ((1024u - (smem_u32(smem) & 1023u)) & 1023u);  // stages; then the partial outputs
+  TreeSmallSmem& sm = *reinterpret_cast<TreeSmallSmem*>(ring + depth * kTreeStageBytes);
+  float* score = reinterpret_cast<float*>(&sm + 1);                    // [group][score_cap]
+  float* op = reinterpret_cast<float*>(ring);                          // [4][RP][kTreeOPitch]
 
   TreeCta c;
   if (!tree_begin<SCORED>(a, c)) return;
   const int warp = c.warp, lane = c.lane, g = lane >> 2, t = lane & 3;
   const int gl = a.group_log2, G = 1 << gl;
   cluster_arrive();
-#pragma unroll
-  for (int j = 0; j < kTreeStages - 1; ++j) {
-    if (j >= c.fresh && j < c.tiles) tree_issue(a, c, smem_u32(ring), j);
-    cp_commit();
+  const uint32_t rg = smem_u32(ring);
+  // one thread copies; a tile with rows behind the cached slots is announced after its V rows there
+  // have been zeroed
+  auto copy = [&](int j) {
+    if (j < c.fresh) return;
+    const int s = j % depth;
+    uint64_t* bar = tree_left(c, j) < kTreeTile ? &sm.tail : &sm.full[s];
+    mbar_expect_tx(bar, kTreeStageBytes);
+    tree_copy(c, &a.km, rg + s * kTreeStageBytes, j, bar);
+    tree_copy(c, &a.vm, rg + s * kTreeStageBytes + kTreeHalf, j, bar);
+  };
+  if (c.tid == 128) {
+    prefetch_tmap(&a.km);
+    prefetch_tmap(&a.vm);
+    for (int i = 0; i < depth; ++i) {
+      mbar_init(&sm.full[i], 1);
+      mbar_init(&sm.empty[i], 4);
+    }
+    mbar_init(&sm.tail, 1);
+    fence_mbar_init();
+    for (int j = 0; j < depth && j < c.tiles; ++j) copy(j);
   }
-  const bool ok = SCORED || tree_ancestors(a, c, anc, up);
+  const bool ok = SCORED || tree_ancestors(a, c, sm.anc, sm.up);
   cluster_wait();  // every CTA of the cluster runs
-  if (!ok) {
-    cp_wait<0>();
-    return;
-  }
-  tree_rows<RP, SCORED>(a, c, anc, qs, ring);
+  if (ok && warp < 4) tree_rows<RP, SCORED>(a, c, sm.anc, sm.q, ring);
+  if (ok && warp == 4 && c.fresh) tree_zero_tail(ring + kTreeHalf, c.n, lane);
   if (c.share) cluster_sync_all();
   else __syncthreads();
+  if (!ok) {  // nothing but the first copies is under way
+    if (c.tid == 128)
+      for (int j = c.fresh; j < depth && j < c.tiles; ++j)
+        mbar_wait_own(tree_left(c, j) < kTreeTile ? &sm.tail : &sm.full[j], 0, a.err, kErrTimeoutFull);
+    return;
+  }
 
   float o[16][4] = {}, m[2] = {-INFINITY, -INFINITY}, l[2] = {};
+  if (warp == 4) {
+    bool run = true;
+    int j = 0;
+    for (; j < c.tiles; ++j) {
+      const int s = j % depth;
+      if (j >= depth) {
+        run &= mbar_wait_own(&sm.empty[s], (j / depth - 1) & 1, a.err, kErrTimeoutEmpty);
+        if (!__all_sync(0xffffffffu, run)) break;
+        if (lane == 0) copy(j);
+      }
+      if (j < c.fresh) {
+        if (lane == 0) mbar_arrive(&sm.full[s]);
+      } else if (tree_left(c, j) < kTreeTile) {
+        mbar_wait_own(&sm.tail, 0, a.err, kErrTimeoutFull);
+        tree_zero_tail(ring + s * kTreeStageBytes + kTreeHalf, (int)tree_left(c, j), lane);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sm.full[s]);
+      }
+    }
+    // the copies under way land before the memory is used again
+    for (int i = j > depth ? j - depth : 0; i < j; ++i)
+      mbar_wait_own(&sm.full[i % depth], (i / depth) & 1, a.err, kErrTimeoutFull);
+  } else {
   uint32_t qf[8][4];
 #pragma unroll
   for (int kk = 0; kk < 8; ++kk)
-    ldsm4(qf[kk], smem_u32(qs) + tile_at<RP>((lane & 7) + ((lane >> 3) & 1) * 8, 2 * kk + (lane >> 4)));
+    ldsm4(qf[kk], smem_u32(sm.q) + tile_at<RP>((lane & 7) + ((lane >> 3) & 1) * 8, 2 * kk + (lane >> 4)));
 
+  bool run = true;
   for (int j = 0; j < c.tiles; ++j) {
-    cp_wait<kTreeStages - 2>();
-    __syncthreads();
-    if (j + kTreeStages - 1 < c.tiles) tree_issue(a, c, smem_u32(ring), j + kTreeStages - 1);
-    cp_commit();
-    const uint32_t st = smem_u32(ring) + (j % kTreeStages) * kTreeStageBytes;
+    const int sl = j % depth;
+    const uint32_t st = rg + sl * kTreeStageBytes;
     const bool fresh = j < c.fresh;
-    const int64_t left = c.len - (int64_t)(c.lo + j - c.fresh) * kTreeTile;
+    const int64_t left = tree_left(c, j);
     const int nv = fresh ? c.n : (int)(left < kTreeTile ? left : kTreeTile);
+    run &= mbar_wait_own(&sm.full[sl], (j / depth) & 1, a.err, kErrTimeoutFull);
+    if (!__all_sync(0xffffffffu, run)) break;
     const int k0 = warp * 16;
-    if (k0 >= nv) continue;
+    if (k0 < nv) {
     float s[2][4] = {};
 #pragma unroll
     for (int kk = 0; kk < 8; ++kk) {
@@ -396,7 +448,7 @@ __global__ void __launch_bounds__(kTreeThreads, 2) k_tree_attn(const TreeArgs a)
     if (fresh || nv < kTreeTile) {
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        const unsigned long long see = tree_seen(c, anc, fresh && !SCORED, g + 8 * e, nv, gl);
+        const unsigned long long see = tree_seen(c, sm.anc, fresh && !SCORED, g + 8 * e, nv, gl);
 #pragma unroll
         for (int i = 0; i < 4; ++i)
           if (!((see >> (k0 + 8 * (i >> 1) + 2 * t + (i & 1))) & 1)) s[i >> 1][2 * e + (i & 1)] = -INFINITY;
@@ -441,33 +493,38 @@ __global__ void __launch_bounds__(kTreeThreads, 2) k_tree_attn(const TreeArgs a)
       mma_16816(o[2 * d], pf[0][0], pf[0][1], pf[1][0], pf[1][1], bf[0], bf[1]);
       mma_16816(o[2 * d + 1], pf[0][0], pf[0][1], pf[1][0], pf[1][1], bf[2], bf[3]);
     }
+    }
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&sm.empty[sl]);
   }
-  cp_wait<0>();
+  }
   __syncthreads();  // the ring becomes the partial outputs
 
+  if (warp < 4) {
 #pragma unroll
   for (int e = 0; e < 2; ++e) {
     const int row = g + 8 * e;
     float s = l[e];
     s = __fadd_rn(s, __shfl_xor_sync(0xffffffffu, s, 1));
     s = __fadd_rn(s, __shfl_xor_sync(0xffffffffu, s, 2));
-    if (t == 0) mlw[warp * RP + row] = make_float2(m[e], s);
+    if (t == 0) sm.mlw[warp][row] = make_float2(m[e], s);
 #pragma unroll
     for (int d = 0; d < 16; ++d)
       *reinterpret_cast<float2*>(op + (warp * RP + row) * kTreeOPitch + 8 * d + 2 * t) =
           make_float2(o[d][2 * e], o[d][2 * e + 1]);
   }
+  }
   __syncthreads();
   // the warps' partials into one per row: a warp a row, four dims a lane
-  for (int r = warp; r < c.R; r += 4) {
+  for (int r = warp; r < c.R && warp < 4; r += 4) {
     float M = -INFINITY, L = 0.0f;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) M = fmaxf(M, mlw[k * RP + r].x);
+    for (int k = 0; k < 4; ++k) M = fmaxf(M, sm.mlw[k][r].x);
     const float mu = M == -INFINITY ? 0.0f : M;
     float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-      const float2 q = mlw[k * RP + r];
+      const float2 q = sm.mlw[k][r];
       const float f = ex2(__fsub_rn(q.x, mu));
       const float4 x = *reinterpret_cast<const float4*>(op + (k * RP + r) * kTreeOPitch + 4 * lane);
       L = __fmaf_rn(q.y, f, L);
@@ -475,10 +532,10 @@ __global__ void __launch_bounds__(kTreeThreads, 2) k_tree_attn(const TreeArgs a)
       s.z = __fmaf_rn(x.z, f, s.z), s.w = __fmaf_rn(x.w, f, s.w);
     }
     *reinterpret_cast<float4*>(op + r * kTreeOPitch + 4 * lane) = s;
-    if (lane == 0) ml[r] = make_float2(M, L);
+    if (lane == 0) sm.ml[r] = make_float2(M, L);
   }
   cluster_sync_all();
-  tree_output(a, c, ml, op);
+  if (warp < 4) tree_output(a, c, sm.ml, op);
   if (SCORED) {
     // each slot's softmax weights of the group's heads join its accumulator, in f32
     float M[8], I[8];
@@ -486,7 +543,7 @@ __global__ void __launch_bounds__(kTreeThreads, 2) k_tree_attn(const TreeArgs a)
     for (int j = 0; j < 8; ++j)
       if (j < G) {
         float L, f;
-        tree_row_total(c, ml, j, M[j], L, f);
+        tree_row_total(c, sm.ml, j, M[j], L, f);
         if (M[j] == -INFINITY) M[j] = 0.0f;
         I[j] = L == 0.0f ? 0.0f : __fdiv_rn(1.0f, L);
       }
@@ -558,111 +615,190 @@ __device__ __forceinline__ uint64_t tree_v_desc(uint32_t saddr) {
   return d;
 }
 
-// TMEM columns: the queries (f16 pairs, the A operand of S = Q K^T), S (f32; its first half then holds
-// the weights as f16 pairs, the A operand of O += P V), and O.  256 in all: two CTAs an SM.
-constexpr uint32_t kTreeTmemCols = 256, kTreeTmemS = 64, kTreeTmemO = 128;
+// TMEM columns: S of even and of odd tiles (f32; the first half then holds the weights as f16 pairs,
+// the A operand of O += P V), and O.  256 in all: two CTAs an SM.
+constexpr uint32_t kTreeTmemCols = 256, kTreeTmemO = 128;
+constexpr int kTreeTcThreads = 192;  // four softmax warps, a copying warp, an MMA warp
 
 struct TreeTcSmem {  // behind the ring
   float2 ml[kTreeRows];
   unsigned long long anc[kTreeMaxTokens];
   int up[kTreeMaxTokens];
-  uint64_t s_done, o_done;
+  uint64_t k_full[kTreeMaxDepth], k_empty[kTreeMaxDepth], v_full[kTreeMaxDepth], v_empty[kTreeMaxDepth];
+  uint64_t s_full[2], p_full[2], o_done, tail;
   uint32_t tmem;
 };
-constexpr size_t kTreeTcBytes = 1024 + kTreeStages * kTreeStageBytes + sizeof(TreeTcSmem);
+constexpr size_t tree_tc_bytes(int depth) {
+  return 1024 + kTreeRows * 256 + (size_t)depth * kTreeStageBytes + sizeof(TreeTcSmem);
+}
 
-// Thread r holds row r's softmax: one TMEM lane, no shuffles.  O stays in TMEM; it is rescaled only
-// when a row's maximum has grown by more than 2^8 since its last reference (the weights, relative to
-// that reference, stay below 2^8 and exact in form; sum and output share the reference).
-// Per tile: S = Q K^T (8 MMAs of 128 x 64 x 16), softmax, O += P V (4 of 128 x 128 x 16), one after the
-// other; the other CTA of the SM fills the gaps.
-__global__ void __launch_bounds__(kTreeThreads, 2) k_tree_tc(const TreeArgs a) {
+// Up to 128 rows, M = 128 whatever the number (padding rows cost nothing that bounds it).  Roles:
+//   copying warp  one thread streams the K and V halves of the tiles into the ring
+//   MMA warp      one thread: S(j) = Q K^T (8 MMAs of 128 x 64 x 16) into one of two S buffers, then,
+//                 when the weights of tile j - 1 are written, O += P V (4 of 128 x 128 x 16); so S(j)
+//                 runs during the softmax of tile j - 1
+//   softmax warps thread r holds row r: one TMEM lane, no shuffles.  O stays in TMEM; it is rescaled
+//                 only when a row's maximum has grown by more than 2^8 over its reference (weights
+//                 relative to it stay below 2^8; sum and output share it, so the quotient is the same)
+__global__ void __launch_bounds__(kTreeTcThreads, 2) k_tree_tc(const __grid_constant__ TreeArgs a, const int depth) {
   extern __shared__ uint8_t smem_raw[];
-  uint8_t* ring = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-  uint8_t* qs = ring + (kTreeStages - 1) * kTreeStageBytes;  // until the queries are in TMEM
-  TreeTcSmem& sm = *reinterpret_cast<TreeTcSmem*>(ring + kTreeStages * kTreeStageBytes);
-  float* op = reinterpret_cast<float*>(ring);                // [rows][kTreeOPitch], at the end
+  uint8_t* qs = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);  // [128][128] f16
+  uint8_t* ring = qs + kTreeRows * 256;
+  TreeTcSmem& sm = *reinterpret_cast<TreeTcSmem*>(ring + depth * kTreeStageBytes);
+  float* op = reinterpret_cast<float*>(qs);  // [rows][kTreeOPitch], at the end
 
   TreeCta c;
   if (!tree_begin<false>(a, c)) return;
-  const int gl = a.group_log2, row = c.tid;
+  const int gl = a.group_log2, row = c.tid, warp = c.warp, lane = c.lane;
+  const uint32_t rg = smem_u32(ring);
   cluster_arrive();
-#pragma unroll
-  for (int j = 0; j < kTreeStages - 1; ++j) {
-    if (j >= c.fresh && j < c.tiles) tree_issue(a, c, smem_u32(ring), j);
-    cp_commit();
+  auto copy_k = [&](int j) {
+    if (j < c.fresh) return;
+    mbar_expect_tx(&sm.k_full[j % depth], kTreeHalf);
+    tree_copy(c, &a.km, rg + (j % depth) * kTreeStageBytes, j, &sm.k_full[j % depth]);
+  };
+  auto copy_v = [&](int j) {  // with rows behind the cached slots: announced after these are zeroed
+    if (j < c.fresh) return;
+    uint64_t* bar = tree_left(c, j) < kTreeTile ? &sm.tail : &sm.v_full[j % depth];
+    mbar_expect_tx(bar, kTreeHalf);
+    tree_copy(c, &a.vm, rg + (j % depth) * kTreeStageBytes + kTreeHalf, j, bar);
+  };
+  if (c.tid == 128) {
+    prefetch_tmap(&a.km);
+    prefetch_tmap(&a.vm);
+    for (int i = 0; i < depth; ++i) {
+      mbar_init(&sm.k_full[i], 1);
+      mbar_init(&sm.k_empty[i], 1);
+      mbar_init(&sm.v_full[i], 1);
+      mbar_init(&sm.v_empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&sm.s_full[i], 1);
+      mbar_init(&sm.p_full[i], (c.R + 31) / 32);
+    }
+    mbar_init(&sm.o_done, 1);
+    mbar_init(&sm.tail, 1);
+    fence_mbar_init();
+    for (int j = 0; j < depth && j < c.tiles; ++j) copy_k(j), copy_v(j);
   }
   const bool tree_ok = tree_ancestors(a, c, sm.anc, sm.up);
   cluster_wait();
   if (!tree_ok) {
-    cp_wait<0>();
+    if (c.tid == 128)
+      for (int j = c.fresh; j < depth && j < c.tiles; ++j) {
+        mbar_wait_own(&sm.k_full[j], 0, a.err, kErrTimeoutFull);
+        mbar_wait_own(tree_left(c, j) < kTreeTile ? &sm.tail : &sm.v_full[j], 0, a.err, kErrTimeoutFull);
+      }
     return;
   }
-  if (c.tid == 0) {
-    mbar_init(&sm.s_done, 1);
-    mbar_init(&sm.o_done, 1);
-    fence_mbar_init();
-  }
-  if (c.warp == 0) {
+  if (warp == 5) {
+    __syncwarp();
     tmem_alloc(&sm.tmem, kTreeTmemCols);
     tmem_relinquish();
   }
-  tree_rows<kTreeRows, false>(a, c, sm.anc, qs, ring);
-  asm volatile("fence.proxy.async;" ::: "memory");  // the new K and V rows, here or in the last CTA, go to MMAs
+  if (warp < 4) {
+    tree_rows<kTreeRows, false>(a, c, sm.anc, qs, ring);
+  }
+  if (warp == 4 && c.fresh) tree_zero_tail(ring + kTreeHalf, c.n, lane);
+  asm volatile("fence.proxy.async;" ::: "memory");  // queries and new rows, here or in a peer, go to MMAs
   tc_fence_before();
   if (c.share) cluster_sync_all();
   else __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = sm.tmem, lane_base = tmem + ((uint32_t)(c.warp * 32) << 16);
-  const bool live = c.warp * 32 < c.R;  // warps of padding rows only copy and wait
-  if (live) {
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      uint32_t q[32];
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const uint4 x = *reinterpret_cast<const uint4*>(qs + tile_at<kTreeRows>(row, 8 * i + k));
-        q[4 * k] = x.x, q[4 * k + 1] = x.y, q[4 * k + 2] = x.z, q[4 * k + 3] = x.w;
-      }
-      tmem_st32(lane_base + 32 * i, q);
-    }
-    tmem_wait_st();
-  }
-
-  constexpr uint32_t kIdS = idesc_f16_f32(128, kTreeTile);
-  constexpr uint32_t kIdO = idesc_f16_f32(128, kHD) | (1u << 16);  // B is MN-major
+  const uint32_t tmem = sm.tmem;
+  const bool live = warp * 32 < c.R;  // softmax warps of padding rows have nothing to do
   float m = -INFINITY, l = 0.0f;
-  bool ok = true;
-  int j = 0;
-  for (; j < c.tiles; ++j) {
-    cp_wait<kTreeStages - 2>();
+
+  if (warp == 4) {
     fence_async_smem();
-    tc_fence_before();
-    __syncthreads();
-    const uint32_t st = smem_u32(ring) + (j % kTreeStages) * kTreeStageBytes;
-    if (c.tid == 0) {
-      tc_fence_after();
-      // P of the tile before shares columns with S
-      if (j > 0) ok &= mbar_wait_own(&sm.o_done, (j - 1) & 1, a.err, kErrTimeoutFull);
-      tc_fence_after();
-#pragma unroll
-      for (int kk = 0; kk < 8; ++kk)
-        umma_f16_ts(tmem + kTreeTmemS, tmem + 8 * kk, sw128_desc(st + (kk >> 2) * (kTreeHalf / 2) + (kk & 3) * 32),
-                    kIdS, kk != 0);
-      umma_commit(&sm.s_done);
+    bool ok = true;
+    int j = 0;
+    for (; j < c.tiles; ++j) {
+      const int s = j % depth;
+      if (j >= depth) {
+        ok &= mbar_wait_own(&sm.k_empty[s], (j / depth - 1) & 1, a.err, kErrTimeoutEmpty);
+        if (!__all_sync(0xffffffffu, ok)) break;
+        if (lane == 0) copy_k(j);
+        ok &= mbar_wait_own(&sm.v_empty[s], (j / depth - 1) & 1, a.err, kErrTimeoutEmpty);
+        if (!__all_sync(0xffffffffu, ok)) {
+          mbar_wait_own(&sm.k_full[s], (j / depth) & 1, a.err, kErrTimeoutFull);
+          break;
+        }
+        if (lane == 0) copy_v(j);
+      }
+      if (j < c.fresh) {
+        if (lane == 0) {
+          mbar_arrive(&sm.k_full[s]);
+          mbar_arrive(&sm.v_full[s]);
+        }
+      } else if (tree_left(c, j) < kTreeTile) {
+        mbar_wait_own(&sm.tail, 0, a.err, kErrTimeoutFull);
+        tree_zero_tail(ring + s * kTreeStageBytes + kTreeHalf, (int)tree_left(c, j), lane);
+        fence_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sm.v_full[s]);
+      }
     }
-    ok &= mbar_wait_own(&sm.s_done, j & 1, a.err, kErrTimeoutFull);
-    tc_fence_after();
-    // the tile before is used up (its MMAs precede S): its stage takes the next copies
-    if (j + kTreeStages - 1 < c.tiles) tree_issue(a, c, smem_u32(ring), j + kTreeStages - 1);
-    cp_commit();
-    if (live) {
+    // the copies under way land before the memory is used again
+    for (int i = j > depth ? j - depth : 0; i < j; ++i) {
+      mbar_wait_own(&sm.k_full[i % depth], (i / depth) & 1, a.err, kErrTimeoutFull);
+      mbar_wait_own(&sm.v_full[i % depth], (i / depth) & 1, a.err, kErrTimeoutFull);
+    }
+  } else if (warp == 5) {
+    if (lane == 0) {
+      constexpr uint32_t kIdS = idesc_f16_f32(128, kTreeTile);
+      constexpr uint32_t kIdO = idesc_f16_f32(128, kHD) | (1u << 16);  // B is MN-major
+      const uint32_t qa = smem_u32(qs);
+      bool ok = true;
+      for (int j = 0; ok && j <= c.tiles; ++j) {
+        if (j < c.tiles) {
+          const int s = j % depth;
+          ok &= mbar_wait_own(&sm.k_full[s], (j / depth) & 1, a.err, kErrTimeoutFull);
+          // the weights of tile j - 2 share this S buffer
+          if (j >= 2) ok &= mbar_wait_own(&sm.o_done, (j - 2) & 1, a.err, kErrTimeoutFull);
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t st = rg + s * kTreeStageBytes;
+#pragma unroll
+          for (int kk = 0; kk < 8; ++kk)
+            umma_f16(tmem + (j & 1) * 64, sw128_desc(qa + (kk >> 2) * (kTreeRows * 128) + (kk & 3) * 32),
+                     sw128_desc(st + (kk >> 2) * (kTreeHalf / 2) + (kk & 3) * 32), kIdS, kk != 0);
+          umma_commit(&sm.s_full[j & 1]);
+          umma_commit(&sm.k_empty[s]);
+        }
+        if (j > 0) {
+          const int i = j - 1, s = i % depth;
+          ok &= mbar_wait_own(&sm.v_full[s], (i / depth) & 1, a.err, kErrTimeoutFull);
+          ok &= mbar_wait_own(&sm.p_full[i & 1], (i >> 1) & 1, a.err, kErrTimeoutFull);
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t sv = rg + s * kTreeStageBytes + kTreeHalf;
+#pragma unroll
+          for (int ks = 0; ks < 4; ++ks)
+            umma_f16_ts(tmem + kTreeTmemO, tmem + (i & 1) * 64 + 8 * ks, tree_v_desc(sv + 2048 * ks), kIdO,
+                        (i | ks) != 0);
+          umma_commit(&sm.o_done);
+          umma_commit(&sm.v_empty[s]);
+        }
+      }
+      // nothing may be in flight when the TMEM goes
+      if (c.tiles > 0) mbar_wait_own(&sm.o_done, (c.tiles - 1) & 1, a.err, kErrTimeoutFull);
+    }
+    __syncwarp();
+  } else if (live) {
+    const uint32_t lane_base = tmem + ((uint32_t)(warp * 32) << 16);
+    bool ok = true;
+    for (int j = 0; j < c.tiles; ++j) {
+      const uint32_t sa = lane_base + (j & 1) * 64;
+      ok &= mbar_wait_own(&sm.s_full[j & 1], (j >> 1) & 1, a.err, kErrTimeoutFull);
+      if (!__all_sync(0xffffffffu, ok)) break;
+      tc_fence_after();
       const bool fresh = j < c.fresh;
-      const int64_t left = c.len - (int64_t)(c.lo + j - c.fresh) * kTreeTile;
+      const int64_t left = tree_left(c, j);
       const int nv = fresh ? c.n : (int)(left < kTreeTile ? left : kTreeTile);
       uint32_t u[64];
-      tmem_ld32(lane_base + kTreeTmemS, u);
-      tmem_ld32(lane_base + kTreeTmemS + 32, u + 32);
+      tmem_ld32(sa, u);
+      tmem_ld32(sa + 32, u + 32);
       tmem_wait_ld();
       if (fresh || nv < kTreeTile) {
         const unsigned long long see = tree_seen(c, sm.anc, fresh, row, nv, gl);
@@ -674,10 +810,13 @@ __global__ void __launch_bounds__(kTreeThreads, 2) k_tree_tc(const TreeArgs a) {
 #pragma unroll
       for (int i = 0; i < 64; ++i) mx[i & 3] = fmaxf(mx[i & 3], __uint_as_float(u[i]));
       const float top = __fmul_rn(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])), kTreeLog2Scale);
-      const bool grow = top > __fadd_rn(m, 8.0f);  // from -inf: the first key that counts
+      const bool grow = row < c.R && top > __fadd_rn(m, 8.0f);  // from -inf: the first key that counts
       const float mn = grow ? top : m;
       const float mu = mn == -INFINITY ? 0.0f : mn;
       if (j > 0 && __any_sync(0xffffffffu, grow)) {
+        ok &= mbar_wait_own(&sm.o_done, (j - 1) & 1, a.err, kErrTimeoutFull);
+        if (!__all_sync(0xffffffffu, ok)) break;
+        tc_fence_after();
         const float al = grow ? ex2(__fsub_rn(m, mu)) : 1.0f;
         l = __fmul_rn(l, al);
 #pragma unroll
@@ -701,25 +840,17 @@ __global__ void __launch_bounds__(kTreeThreads, 2) k_tree_tc(const TreeArgs a) {
         p[i] = pack_h2(p0, p1);
       }
       l = __fadd_rn(l, __fadd_rn(__fadd_rn(sum[0], sum[1]), __fadd_rn(sum[2], sum[3])));
-      tmem_st32(lane_base + kTreeTmemS, p);
+      tmem_st32(sa, p);
       tmem_wait_st();
-    }
-    tc_fence_before();
-    if (__syncthreads_or(!ok)) break;
-    if (c.tid == 0) {
-      tc_fence_after();
-#pragma unroll
-      for (int ks = 0; ks < 4; ++ks)
-        umma_f16_ts(tmem + kTreeTmemO, tmem + kTreeTmemS + 8 * ks, tree_v_desc(st + kTreeHalf + 2048 * ks), kIdO,
-                    (j | ks) != 0);
-      umma_commit(&sm.o_done);
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sm.p_full[j & 1]);
     }
   }
-  cp_wait<0>();
-  if (j > 0) mbar_wait_own(&sm.o_done, (j - 1) & 1, a.err, kErrTimeoutFull);
+  __syncthreads();  // all MMAs and copies are done: the operands' memory becomes the partial outputs
   tc_fence_after();
-  __syncthreads();  // the ring becomes the partial outputs
-  if (live) {
+  if (warp < 4 && live) {
+    const uint32_t lane_base = tmem + ((uint32_t)(warp * 32) << 16);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       uint32_t x[32];
@@ -736,11 +867,11 @@ __global__ void __launch_bounds__(kTreeThreads, 2) k_tree_tc(const TreeArgs a) {
   }
   tc_fence_before();
   cluster_sync_all();
-  if (c.warp == 0) {
+  if (warp == 5) {
     tc_fence_after();
     tmem_dealloc(tmem, kTreeTmemCols);
   }
-  tree_output(a, c, sm.ml, op);
+  if (warp < 4) tree_output(a, c, sm.ml, op);
   cluster_sync_all();  // peers read this CTA's shared memory until here
 }
 
