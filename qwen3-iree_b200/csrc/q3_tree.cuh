@@ -123,7 +123,8 @@ struct TreeCta {
 template <bool SCORED>
 __device__ __forceinline__ bool tree_begin(const TreeArgs& a, TreeCta& c) {
   c.C = gridDim.x, c.rank = blockIdx.x, c.h = blockIdx.y, c.b = blockIdx.z;
-  c.tid = threadIdx.x, c.warp = c.tid >> 5, c.lane = c.tid & 31;
+  c.tid = threadIdx.x, c.lane = c.tid & 31;
+  c.warp = __shfl_sync(0xffffffffu, c.tid >> 5, 0);  // uniform for the compiler too
   c.n = SCORED ? 1 : (a.n_tokens ? a.n_tokens[c.b] : a.T);
   c.len = a.len[c.b], c.pos = a.pos[c.b];
   if (SCORED ? c.len == -1 : c.n == 0) return false;
@@ -580,6 +581,12 @@ __device__ __forceinline__ void umma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, ui
       "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
       : "memory");
 }
+// One lane of a converged warp.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t e;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(e));
+  return e != 0;
+}
 // 32 consecutive columns of this thread's TMEM lane to / from registers.
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t* r) {
   asm volatile(
@@ -745,45 +752,54 @@ __global__ void __launch_bounds__(kTreeTcThreads, 2) k_tree_tc(const __grid_cons
       mbar_wait_own(&sm.v_full[i % depth], (i / depth) & 1, a.err, kErrTimeoutFull);
     }
   } else if (warp == 5) {
-    if (lane == 0) {
-      constexpr uint32_t kIdS = idesc_f16_f32(128, kTreeTile);
-      constexpr uint32_t kIdO = idesc_f16_f32(128, kHD) | (1u << 16);  // B is MN-major
-      const uint32_t qa = smem_u32(qs);
-      bool ok = true;
-      for (int j = 0; ok && j <= c.tiles; ++j) {
-        if (j < c.tiles) {
-          const int s = j % depth;
-          ok &= mbar_wait_own(&sm.k_full[s], (j / depth) & 1, a.err, kErrTimeoutFull);
-          // the weights of tile j - 2 share this S buffer
-          if (j >= 2) ok &= mbar_wait_own(&sm.o_done, (j - 2) & 1, a.err, kErrTimeoutFull);
-          if (!ok) break;
-          tc_fence_after();
-          const uint32_t st = rg + s * kTreeStageBytes;
+    // the whole warp runs the loop, so that descriptors stay in uniform registers (with one lane in
+    // the loop, moving them there took 80 cycles an MMA); one lane issues
+    constexpr uint32_t kIdS = idesc_f16_f32(128, kTreeTile);
+    constexpr uint32_t kIdO = idesc_f16_f32(128, kHD) | (1u << 16);  // B is MN-major
+    const uint64_t qd = sw128_desc(smem_u32(qs)), kd = sw128_desc(rg), vd = tree_v_desc(rg + kTreeHalf);
+    const bool leader = elect_one();
+    bool ok = true;
+    int s = 0, sp = 0;            // stages of tiles j and j - 1
+    uint32_t ph = 0, php = 0;     // their phases
+    for (int j = 0; j <= c.tiles; ++j) {
+      if (j < c.tiles) {
+        ok &= mbar_wait_own(&sm.k_full[s], ph, a.err, kErrTimeoutFull);
+        // the weights of tile j - 2 share this S buffer
+        if (j >= 2) ok &= mbar_wait_own(&sm.o_done, j & 1, a.err, kErrTimeoutFull);
+        if (!__all_sync(0xffffffffu, ok)) break;
+        tc_fence_after();
+        if (leader) {
+          const uint64_t kj = kd + (uint64_t)(s * (kTreeStageBytes >> 4));
 #pragma unroll
           for (int kk = 0; kk < 8; ++kk)
-            umma_f16(tmem + (j & 1) * 64, sw128_desc(qa + (kk >> 2) * (kTreeRows * 128) + (kk & 3) * 32),
-                     sw128_desc(st + (kk >> 2) * (kTreeHalf / 2) + (kk & 3) * 32), kIdS, kk != 0);
+            umma_f16(tmem + (j & 1) * 64, qd + ((kk >> 2) * (kTreeRows * 128) + (kk & 3) * 32) / 16,
+                     kj + ((kk >> 2) * (kTreeHalf / 2) + (kk & 3) * 32) / 16, kIdS, kk != 0);
           umma_commit(&sm.s_full[j & 1]);
           umma_commit(&sm.k_empty[s]);
         }
-        if (j > 0) {
-          const int i = j - 1, s = i % depth;
-          ok &= mbar_wait_own(&sm.v_full[s], (i / depth) & 1, a.err, kErrTimeoutFull);
-          ok &= mbar_wait_own(&sm.p_full[i & 1], (i >> 1) & 1, a.err, kErrTimeoutFull);
-          if (!ok) break;
-          tc_fence_after();
-          const uint32_t sv = rg + s * kTreeStageBytes + kTreeHalf;
+        __syncwarp();
+      }
+      if (j > 0) {
+        const int i = j - 1;
+        ok &= mbar_wait_own(&sm.v_full[sp], php, a.err, kErrTimeoutFull);
+        ok &= mbar_wait_own(&sm.p_full[i & 1], (i >> 1) & 1, a.err, kErrTimeoutFull);
+        if (!__all_sync(0xffffffffu, ok)) break;
+        tc_fence_after();
+        if (leader) {
+          const uint64_t vi = vd + (uint64_t)(sp * (kTreeStageBytes >> 4));
 #pragma unroll
           for (int ks = 0; ks < 4; ++ks)
-            umma_f16_ts(tmem + kTreeTmemO, tmem + (i & 1) * 64 + 8 * ks, tree_v_desc(sv + 2048 * ks), kIdO,
-                        (i | ks) != 0);
+            umma_f16_ts(tmem + kTreeTmemO, tmem + (i & 1) * 64 + 8 * ks, vi + 2048 * ks / 16, kIdO, (i | ks) != 0);
           umma_commit(&sm.o_done);
-          umma_commit(&sm.v_empty[s]);
+          umma_commit(&sm.v_empty[sp]);
         }
+        __syncwarp();
       }
-      // nothing may be in flight when the TMEM goes
-      if (c.tiles > 0) mbar_wait_own(&sm.o_done, (c.tiles - 1) & 1, a.err, kErrTimeoutFull);
+      sp = s, php = ph;
+      if (++s == depth) s = 0, ph ^= 1;
     }
+    // nothing may be in flight when the TMEM goes
+    if (c.tiles > 0) mbar_wait_own(&sm.o_done, (c.tiles - 1) & 1, a.err, kErrTimeoutFull);
     __syncwarp();
   } else if (live) {
     const uint32_t lane_base = tmem + ((uint32_t)(warp * 32) << 16);
