@@ -544,7 +544,7 @@ int q3_tree_commit(const q3_kv_cache* cache, int layer0, int n_layers, int B, in
  *   weight, new_weight: f32 [B][layers][kv_heads][slots], the same array or
  *             apart; slot_pos: int32 of that shape, the position each slot holds
  *   len:      -1 skips the sequence.
- * slots up to 180,224 with two query heads per kv head (their scores stay on
+ * slots up to 180,160 with two query heads per kv head (their scores stay on
  * chip), in inverse proportion to that number. */
 int q3_decode_attention_scored(const void* qkv, const void* q_norm, const void* k_norm,
                                const float* rope_cos, const float* rope_sin, int64_t rope_rows,

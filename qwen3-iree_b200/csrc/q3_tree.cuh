@@ -32,9 +32,10 @@ constexpr int kTreeTile = 64;                             // keys per ring stage
 constexpr int kTreeHalf = kTreeTile * kHD * 2;            // a stage: K, then V
 constexpr int kTreeStageBytes = 2 * kTreeHalf;
 constexpr int kTreeOPitch = kHD + 4;                      // floats between partial output rows
+constexpr int kTreeMaxCluster = 16;
 constexpr int kTreeMaxDepth = 6;                          // tiles a ring holds
 constexpr int kTreeSmallRows = 16;                        // rows of k_tree_attn
-constexpr int kTreeRows = 128;                            // rows of k_tree_tc
+constexpr int kTreeRows = 128;                            // most rows of k_tree_tc
 constexpr float kTreeLog2Scale = kAttnScale * 1.44269504088896341f;  // scores in powers of two
 
 struct TreeArgs {
@@ -117,6 +118,7 @@ struct TreeCta {
   int64_t len, pos;                 // fresh: 1 in the last CTA, whose tile 0 holds the new tokens
   uint16_t *kb, *vb;
   bool share;                       // the cluster's CTAs prepare the query rows for one another
+  int parent;                       // of token `tid`
 };
 
 // Reads and checks the sequence's values; false: nothing to do (the same in all CTAs of a cluster).
@@ -127,6 +129,7 @@ __device__ __forceinline__ bool tree_begin(const TreeArgs& a, TreeCta& c) {
   c.warp = __shfl_sync(0xffffffffu, c.tid >> 5, 0);  // uniform for the compiler too
   c.n = SCORED ? 1 : (a.n_tokens ? a.n_tokens[c.b] : a.T);
   c.len = a.len[c.b], c.pos = a.pos[c.b];
+  c.parent = !SCORED && c.tid < a.T ? a.parents[(int64_t)c.b * a.T + c.tid] : -1;
   if (SCORED ? c.len == -1 : c.n == 0) return false;
   if (c.n < 0 || c.n > a.T || c.len < 0 || c.len > a.S - c.n || c.pos < 0 || c.pos >= a.rope_rows) {
     if (c.tid == 0 && a.err) atomicCAS(a.err, 0, kErrBadPos);
@@ -140,7 +143,7 @@ __device__ __forceinline__ bool tree_begin(const TreeArgs& a, TreeCta& c) {
   c.fresh = c.rank == c.C - 1;
   c.kb = a.k + c.b * a.seq_stride + c.h * a.head_stride;
   c.vb = a.v + c.b * a.seq_stride + c.h * a.head_stride;
-  c.share = c.C > 1 && c.R > 8;
+  c.share = c.C > 1 && c.R > kTreeSmallRows;  // below, pushing them costs more than preparing them
   return true;
 }
 
@@ -165,44 +168,53 @@ __device__ __forceinline__ void tree_copy(const TreeCta& c, const CUtensorMap* m
   tma_load_4d(dst + kTreeHalf / 2, map, 64, slot, c.h, c.b, bar);
 }
 
-// Ancestors by doubling: after each step a token knows twice as many.  anc[i]: ancestors of i and i
-// itself; up: scratch.  false: a bad tree, or a token beyond the RoPE tables.
+// Ancestors by doubling, until the deepest token has met the root: after each step a token knows twice
+// as many.  anc[i]: ancestors of i and i itself; up: scratch.  false: a bad tree, or a token beyond the
+// RoPE tables.
 __device__ __forceinline__ bool tree_ancestors(const TreeArgs& a, const TreeCta& c,
                                                unsigned long long* anc, int* up) {
-  bool ok = true;
-  if (c.tid < c.n) {
-    const int p = a.parents[(int64_t)c.b * a.T + c.tid];
-    ok = p >= -1 && p < c.tid;
-    up[c.tid] = ok ? p : -1;
-    anc[c.tid] = 1ull << c.tid;
-  }
-  if (__syncthreads_or(!ok)) {
+  const bool mine = c.tid < c.n;
+  int u = c.parent;
+  unsigned long long m = 1ull << (c.tid & 63);
+  if (mine) up[c.tid] = u, anc[c.tid] = m;
+  if (__syncthreads_or(mine && (u < -1 || u >= c.tid))) {
     if (c.tid == 0 && a.err) atomicCAS(a.err, 0, kErrBadTree);
     return false;
   }
-  for (int s = 1; s < c.n; s <<= 1) {
-    unsigned long long m = 0;
-    int u = -1;
-    if (c.tid < c.n && up[c.tid] >= 0) m = anc[up[c.tid]], u = up[up[c.tid]];
-    __syncthreads();
-    if (c.tid < c.n) anc[c.tid] |= m, up[c.tid] = u;
+  while (true) {
+    const bool more = mine && u >= 0;
+    if (more) m |= anc[u], u = up[u];
+    if (!__syncthreads_or(more)) break;
+    if (more) anc[c.tid] = m, up[c.tid] = u;
     __syncthreads();
   }
-  if (__syncthreads_or(c.tid < c.n && c.pos + __popcll(anc[c.tid]) - 1 >= a.rope_rows)) {
+  if (__syncthreads_or(mine && c.pos + __popcll(m) - 1 >= a.rope_rows)) {
     if (c.tid == 0 && a.err) atomicCAS(a.err, 0, kErrBadPos);
     return false;
   }
   return true;
 }
 
+// v / r, correctly rounded, from y = 1 / r correctly rounded (Markstein, IBM J. Res. Dev. 34, 1990):
+// q = v y is within an ulp, its remainder v - q r is exact in one fma, and one more fma rounds the
+// corrected quotient as a division would.  Where r is infinite (y = 0) q itself is the answer.  Needs
+// no underflow: here |v| >= 2^-24 or 0, and 2^-10 <= r <= 2^16.
+__device__ __forceinline__ float div_by(float v, float r, float y) {
+  const float q = __fmul_rn(v, y);
+  const float c = __fmaf_rn(__fmaf_rn(-q, r, v), y, q);
+  return y == 0.0f ? q : c;
+}
+
 // QK-RMSNorm and RoPE of the query rows into the tile `qs` (ROWS rows) of every CTA, and of the new K
-// rows, with the V rows as they are, into stage 0 of the last CTA and into the cache.  The operations
-// and roundings of norm_rope_vals, a warp per row, two rows at a time.  With `share` the rows are
+// rows, with the V rows as they are, into the first tile of the last CTA and into the cache.  The operations
+// and roundings of norm_rope_vals, a warp per row, E rows at a time without branches between them (its
+// divisions branch, and took most of 0.35 us a row).  With `share` the rows are
 // dealt out to the cluster's CTAs, which push them to one another (the caller has waited until all
 // CTAs run, and follows with a cluster barrier); otherwise each CTA prepares all it needs.
-template <int ROWS, bool SCORED>
+template <int ROWS, int WARPS, int E, bool SCORED>
 __device__ __forceinline__ void tree_rows(const TreeArgs& a, const TreeCta& c,
-                                          const unsigned long long* anc, uint8_t* qs, uint8_t* ring) {
+                                          const unsigned long long* anc, uint8_t* qs, uint8_t* knew,
+                                          uint8_t* vnew) {
   const int gl = a.group_log2, lane = c.lane;
   const int64_t row_el = (int64_t)(a.q_heads + 2 * a.kv_heads) * kHD;
   const uint16_t* qkv = a.qkv + (int64_t)c.b * a.T * row_el;
@@ -210,13 +222,13 @@ __device__ __forceinline__ void tree_rows(const TreeArgs& a, const TreeCta& c,
 #pragma unroll
   for (int i = 0; i < 4; ++i) gq[i] = h2f(a.q_norm[lane + 32 * i]), gk[i] = h2f(a.k_norm[lane + 32 * i]);
   const int units = c.share || c.fresh ? c.R + c.n : c.R;
-  const int step = c.share ? 4 * c.C : 4;
+  const int step = c.share ? WARPS * c.C : WARPS;
   const int last = c.C - 1;
-  for (int u0 = c.share ? c.rank + c.C * c.warp : c.warp; u0 < units; u0 += 2 * step) {
-    float v[2][4], cs[2][4];
-    uint2 vv[2];
+  for (int u0 = c.share ? c.rank + c.C * c.warp : c.warp; u0 < units; u0 += E * step) {
+    float v[E][4], cs[E][4];
+    uint2 vv[E];
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
+    for (int e = 0; e < E; ++e) {
       const int u = min(u0 + e * step, units - 1);  // a repeated row is computed and dropped
       const bool isq = u < c.R;
       const int tok = isq ? u >> gl : u - c.R;
@@ -229,36 +241,39 @@ __device__ __forceinline__ void tree_rows(const TreeArgs& a, const TreeCta& c,
       cs[e][0] = a.rope_cos[p], cs[e][1] = a.rope_cos[p + 32];
       cs[e][2] = a.rope_sin[p], cs[e][3] = a.rope_sin[p + 32];
     }
-    float ss[2] = {0.0f, 0.0f};
+    float ss[E] = {};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      ss[0] = __fmaf_rn(v[0][i], v[0][i], ss[0]);
-      ss[1] = __fmaf_rn(v[1][i], v[1][i], ss[1]);
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int e = 0; e < E; ++e) ss[e] = __fmaf_rn(v[e][i], v[e][i], ss[e]);
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1)
+#pragma unroll
+      for (int e = 0; e < E; ++e) ss[e] = __fadd_rn(ss[e], __shfl_xor_sync(0xffffffffu, ss[e], off));
+    uint16_t o[E][4];
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const bool isq = u0 + e * step < c.R;
+      const float r = __fsqrt_rn(__fadd_rn(__fmul_rn(ss[e], 0.0078125f), kEps));
+      const float y = __frcp_rn(r);
+      float x[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[i] = h2f(f2h(__fmul_rn(div_by(v[e][i], r, y), isq ? gq[i] : gk[i])));
+      o[e][0] = f2h(__fsub_rn(__fmul_rn(x[0], cs[e][0]), __fmul_rn(x[2], cs[e][2])));
+      o[e][2] = f2h(__fadd_rn(__fmul_rn(x[0], cs[e][2]), __fmul_rn(x[2], cs[e][0])));
+      o[e][1] = f2h(__fsub_rn(__fmul_rn(x[1], cs[e][1]), __fmul_rn(x[3], cs[e][3])));
+      o[e][3] = f2h(__fadd_rn(__fmul_rn(x[1], cs[e][3]), __fmul_rn(x[3], cs[e][1])));
     }
 #pragma unroll
-    for (int off = 16; off > 0; off >>= 1) {
-      const float y0 = __shfl_xor_sync(0xffffffffu, ss[0], off), y1 = __shfl_xor_sync(0xffffffffu, ss[1], off);
-      ss[0] = __fadd_rn(ss[0], y0), ss[1] = __fadd_rn(ss[1], y1);
-    }
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
+    for (int e = 0; e < E; ++e) {
       const int u = u0 + e * step;
       if (u >= units) break;
       const bool isq = u < c.R;
-      const float r = __fsqrt_rn(__fadd_rn(__fdiv_rn(ss[e], 128.0f), kEps));
-      float x[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) x[i] = h2f(f2h(__fmul_rn(__fdiv_rn(v[e][i], r), isq ? gq[i] : gk[i])));
-      uint16_t o[4];
-      o[0] = f2h(__fsub_rn(__fmul_rn(x[0], cs[e][0]), __fmul_rn(x[2], cs[e][2])));
-      o[2] = f2h(__fadd_rn(__fmul_rn(x[0], cs[e][2]), __fmul_rn(x[2], cs[e][0])));
-      o[1] = f2h(__fsub_rn(__fmul_rn(x[1], cs[e][1]), __fmul_rn(x[3], cs[e][3])));
-      o[3] = f2h(__fadd_rn(__fmul_rn(x[1], cs[e][3]), __fmul_rn(x[3], cs[e][1])));
       if (isq) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int d = lane + 32 * i;
-          *reinterpret_cast<uint16_t*>(qs + tile_at<ROWS>(u, d >> 3) + (d & 7) * 2) = o[i];
+          *reinterpret_cast<uint16_t*>(qs + tile_at<ROWS>(u, d >> 3) + (d & 7) * 2) = o[e][i];
         }
         if (c.share) {  // half a warp a peer
           __syncwarp();
@@ -271,12 +286,12 @@ __device__ __forceinline__ void tree_rows(const TreeArgs& a, const TreeCta& c,
         const int k = u - c.R;
         uint16_t* kd = c.kb + (c.len + k) * a.slot_stride;
         *reinterpret_cast<uint2*>(c.vb + (c.len + k) * a.slot_stride + lane * 4) = vv[e];
-        st_dsmem_v2(smem_u32(ring) + kTreeHalf + tile_at<kTreeTile>(k, lane >> 1) + (lane & 1) * 8, last, vv[e]);
+        st_dsmem_v2(smem_u32(vnew) + tile_at<kTreeTile>(k, lane >> 1) + (lane & 1) * 8, last, vv[e]);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int d = lane + 32 * i;
-          kd[d] = o[i];
-          st_dsmem_u16(smem_u32(ring) + tile_at<kTreeTile>(k, d >> 3) + (d & 7) * 2, last, o[i]);
+          kd[d] = o[e][i];
+          st_dsmem_u16(smem_u32(knew) + tile_at<kTreeTile>(k, d >> 3) + (d & 7) * 2, last, o[e][i]);
         }
       }
     }
@@ -314,17 +329,21 @@ __device__ __forceinline__ void tree_row_total(const TreeCta& c, const float2* m
 // c + C, ..., a warp a row, four dims a lane.
 __device__ __forceinline__ void tree_output(const TreeArgs& a, const TreeCta& c, const float2* ml,
                                             const float* op) {
-  const int gl = a.group_log2, G = 1 << gl;
-  for (int r = c.rank + c.C * c.warp; r < c.R; r += c.C * 4) {
+  const int gl = a.group_log2, G = 1 << gl, warps = blockDim.x >> 5;
+  for (int r = c.rank + c.C * c.warp; r < c.R; r += c.C * warps) {
+    float4 x[kTreeMaxCluster];  // all under way before the factors are known
+#pragma unroll
+    for (int k = 0; k < kTreeMaxCluster; ++k)
+      if (k < c.C) x[k] = ld_dsmem_f4(smem_u32(op + r * kTreeOPitch + 4 * c.lane), k);
     float M, L, f;
     tree_row_total(c, ml, r, M, L, f);
     float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 4
-    for (int k = 0; k < c.C; ++k) {
+#pragma unroll
+    for (int k = 0; k < kTreeMaxCluster; ++k) {
+      if (k >= c.C) break;
       const float fk = __shfl_sync(0xffffffffu, f, k);
-      const float4 x = ld_dsmem_f4(smem_u32(op + r * kTreeOPitch + 4 * c.lane), k);
-      s.x = __fmaf_rn(x.x, fk, s.x), s.y = __fmaf_rn(x.y, fk, s.y);
-      s.z = __fmaf_rn(x.z, fk, s.z), s.w = __fmaf_rn(x.w, fk, s.w);
+      s.x = __fmaf_rn(x[k].x, fk, s.x), s.y = __fmaf_rn(x[k].y, fk, s.y);
+      s.z = __fmaf_rn(x[k].z, fk, s.z), s.w = __fmaf_rn(x[k].w, fk, s.w);
     }
     const float inv = L == 0.0f ? 0.0f : __fdiv_rn(1.0f, L);  // a row that sees nothing is zero
     const uint2 w = make_uint2(pack_h2(__fmul_rn(s.x, inv), __fmul_rn(s.y, inv)),
@@ -358,6 +377,7 @@ __global__ void __launch_bounds__(kTreeThreads, 3)
   float* score = reinterpret_cast<float*>(&sm + 1);                    // [group][score_cap]
   float* op = reinterpret_cast<float*>(ring);                          // [4][RP][kTreeOPitch]
 
+  if (threadIdx.x == 128) prefetch_tmap(&a.km), prefetch_tmap(&a.vm);
   TreeCta c;
   if (!tree_begin<SCORED>(a, c)) return;
   const int warp = c.warp, lane = c.lane, g = lane >> 2, t = lane & 3;
@@ -375,8 +395,6 @@ __global__ void __launch_bounds__(kTreeThreads, 3)
     tree_copy(c, &a.vm, rg + s * kTreeStageBytes + kTreeHalf, j, bar);
   };
   if (c.tid == 128) {
-    prefetch_tmap(&a.km);
-    prefetch_tmap(&a.vm);
     for (int i = 0; i < depth; ++i) {
       mbar_init(&sm.full[i], 1);
       mbar_init(&sm.empty[i], 4);
@@ -387,7 +405,7 @@ __global__ void __launch_bounds__(kTreeThreads, 3)
   }
   const bool ok = SCORED || tree_ancestors(a, c, sm.anc, sm.up);
   cluster_wait();  // every CTA of the cluster runs
-  if (ok && warp < 4) tree_rows<RP, SCORED>(a, c, sm.anc, sm.q, ring);
+  if (ok) tree_rows<RP, 5, SCORED ? 1 : 5, SCORED>(a, c, sm.anc, sm.q, ring, ring + kTreeHalf);
   if (ok && warp == 4 && c.fresh) tree_zero_tail(ring + kTreeHalf, c.n, lane);
   if (c.share) cluster_sync_all();
   else __syncthreads();
@@ -536,7 +554,7 @@ __global__ void __launch_bounds__(kTreeThreads, 3)
     if (lane == 0) sm.ml[r] = make_float2(M, L);
   }
   cluster_sync_all();
-  if (warp < 4) tree_output(a, c, sm.ml, op);
+  tree_output(a, c, sm.ml, op);
   if (SCORED) {
     // each slot's softmax weights of the group's heads join its accumulator, in f32
     float M[8], I[8];
@@ -551,12 +569,23 @@ __global__ void __launch_bounds__(kTreeThreads, 3)
     const int64_t w0 = c.b * a.w_stride + (int64_t)c.h * a.S, s0 = (int64_t)c.lo * kTreeTile;
     const int64_t span = (int64_t)(c.tiles - c.fresh) * kTreeTile, left = c.len - s0;
     const int held = (int)(left < span ? left : span), first = c.fresh * kTreeTile;
-    for (int i = c.tid; i < held; i += kTreeThreads) {
-      float w = a.w_in[w0 + s0 + i];
+    for (int i0 = c.tid; i0 < held; i0 += 8 * kTreeThreads) {
+      float w[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (j < G) w = __fmaf_rn(ex2(__fmaf_rn(score[j * a.score_cap + first + i], kTreeLog2Scale, -M[j])), I[j], w);
-      a.w_out[w0 + s0 + i] = w;
+      for (int k = 0; k < 8; ++k) {
+        const int i = i0 + k * kTreeThreads;
+        if (i < held) w[k] = a.w_in[w0 + s0 + i];
+      }
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const int i = i0 + k * kTreeThreads;
+        if (i >= held) break;
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (j < G)
+            w[k] = __fmaf_rn(ex2(__fmaf_rn(score[j * a.score_cap + first + i], kTreeLog2Scale, -M[j])), I[j], w[k]);
+        a.w_out[w0 + s0 + i] = w[k];
+      }
     }
     if (c.fresh && c.tid == 0) {  // the new slot starts with its own weight
       float w = 0.0f;
@@ -626,18 +655,29 @@ __device__ __forceinline__ uint64_t tree_v_desc(uint32_t saddr) {
 // the A operand of O += P V), and O.  256 in all: two CTAs an SM.
 constexpr uint32_t kTreeTmemCols = 256, kTreeTmemO = 128;
 constexpr int kTreeTcThreads = 192;  // four softmax warps, a copying warp, an MMA warp
+constexpr int kTreeMaxSlots = 3;     // K or V halves of tiles in flight
+// Two CTAs an SM leave 113 KB each: the queries (ROWS rows, 64 or 128) and five or six halves.
+template <int ROWS>
+struct TreeTc {
+  static constexpr int kSlots = 3, vSlots = ROWS == 64 ? 3 : 2;
+  static constexpr int q_bytes = ROWS * 256;
+  static constexpr int op_bytes = ROWS * kTreeOPitch * 4;  // partial outputs, over all of it at the end
+  static constexpr int ring_bytes = (kSlots + vSlots) * kTreeHalf;
+  static_assert(op_bytes + ROWS * 8 <= q_bytes + ring_bytes, "");
+};
 
 struct TreeTcSmem {  // behind the ring
-  float2 ml[kTreeRows];
   unsigned long long anc[kTreeMaxTokens];
   int up[kTreeMaxTokens];
-  uint64_t k_full[kTreeMaxDepth], k_empty[kTreeMaxDepth], v_full[kTreeMaxDepth], v_empty[kTreeMaxDepth];
+  uint64_t k_full[kTreeMaxSlots], k_empty[kTreeMaxSlots], v_full[kTreeMaxSlots], v_empty[kTreeMaxSlots];
   uint64_t s_full[2], p_full[2], o_done, tail;
   uint32_t tmem;
 };
-constexpr size_t tree_tc_bytes(int depth) {
-  return 1024 + kTreeRows * 256 + (size_t)depth * kTreeStageBytes + sizeof(TreeTcSmem);
+template <int ROWS>
+constexpr size_t tree_tc_bytes() {
+  return TreeTc<ROWS>::q_bytes + TreeTc<ROWS>::ring_bytes + sizeof(TreeTcSmem);
 }
+static_assert(tree_tc_bytes<128>() <= 233472 / 2 - 1024 && tree_tc_bytes<64>() <= 233472 / 2 - 1024, "two CTAs an SM");
 
 // Up to 128 rows, M = 128 whatever the number (padding rows cost nothing that bounds it).  Roles:
 //   copying warp  one thread streams the K and V halves of the tiles into the ring
@@ -647,33 +687,41 @@ constexpr size_t tree_tc_bytes(int depth) {
 //   softmax warps thread r holds row r: one TMEM lane, no shuffles.  O stays in TMEM; it is rescaled
 //                 only when a row's maximum has grown by more than 2^8 over its reference (weights
 //                 relative to it stay below 2^8; sum and output share it, so the quotient is the same)
-__global__ void __launch_bounds__(kTreeTcThreads, 2) k_tree_tc(const __grid_constant__ TreeArgs a, const int depth) {
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* qs = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);  // [128][128] f16
-  uint8_t* ring = qs + kTreeRows * 256;
-  TreeTcSmem& sm = *reinterpret_cast<TreeTcSmem*>(ring + depth * kTreeStageBytes);
-  float* op = reinterpret_cast<float*>(qs);  // [rows][kTreeOPitch], at the end
+template <int ROWS>
+__global__ void __launch_bounds__(kTreeTcThreads, 2) k_tree_tc(const __grid_constant__ TreeArgs a) {
+  using L = TreeTc<ROWS>;
+  constexpr int KD = L::kSlots, VD = L::vSlots;
+  extern __shared__ __align__(1024) uint8_t smem_tc[];
+  uint8_t* qs = smem_tc;  // [ROWS][128] f16; an A operand of 128 rows reads on into the ring
+  uint8_t* kring = qs + L::q_bytes;
+  uint8_t* vring = kring + KD * kTreeHalf;
+  TreeTcSmem& sm = *reinterpret_cast<TreeTcSmem*>(vring + VD * kTreeHalf);
+  float* op = reinterpret_cast<float*>(qs);                    // [ROWS][kTreeOPitch], at the end
+  float2* ml = reinterpret_cast<float2*>(qs + L::op_bytes);    // [ROWS]
+  if (smem_u32(smem_tc) & 1023u) {  // the swizzle goes by address bits; no launch here breaks it
+    if (threadIdx.x == 0 && a.err) atomicCAS(a.err, 0, kErrTimeoutFull);
+    return;
+  }
 
+  if (threadIdx.x == 128) prefetch_tmap(&a.km), prefetch_tmap(&a.vm);
   TreeCta c;
   if (!tree_begin<false>(a, c)) return;
   const int gl = a.group_log2, row = c.tid, warp = c.warp, lane = c.lane;
-  const uint32_t rg = smem_u32(ring);
+  const uint32_t kr = smem_u32(kring), vr = smem_u32(vring);
   cluster_arrive();
   auto copy_k = [&](int j) {
     if (j < c.fresh) return;
-    mbar_expect_tx(&sm.k_full[j % depth], kTreeHalf);
-    tree_copy(c, &a.km, rg + (j % depth) * kTreeStageBytes, j, &sm.k_full[j % depth]);
+    mbar_expect_tx(&sm.k_full[j % KD], kTreeHalf);
+    tree_copy(c, &a.km, kr + (j % KD) * kTreeHalf, j, &sm.k_full[j % KD]);
   };
   auto copy_v = [&](int j) {  // with rows behind the cached slots: announced after these are zeroed
     if (j < c.fresh) return;
-    uint64_t* bar = tree_left(c, j) < kTreeTile ? &sm.tail : &sm.v_full[j % depth];
+    uint64_t* bar = tree_left(c, j) < kTreeTile ? &sm.tail : &sm.v_full[j % VD];
     mbar_expect_tx(bar, kTreeHalf);
-    tree_copy(c, &a.vm, rg + (j % depth) * kTreeStageBytes + kTreeHalf, j, bar);
+    tree_copy(c, &a.vm, vr + (j % VD) * kTreeHalf, j, bar);
   };
   if (c.tid == 128) {
-    prefetch_tmap(&a.km);
-    prefetch_tmap(&a.vm);
-    for (int i = 0; i < depth; ++i) {
+    for (int i = 0; i < kTreeMaxSlots; ++i) {
       mbar_init(&sm.k_full[i], 1);
       mbar_init(&sm.k_empty[i], 1);
       mbar_init(&sm.v_full[i], 1);
@@ -686,15 +734,18 @@ __global__ void __launch_bounds__(kTreeTcThreads, 2) k_tree_tc(const __grid_cons
     mbar_init(&sm.o_done, 1);
     mbar_init(&sm.tail, 1);
     fence_mbar_init();
-    for (int j = 0; j < depth && j < c.tiles; ++j) copy_k(j), copy_v(j);
+    for (int j = 0; j < KD && j < c.tiles; ++j) {
+      copy_k(j);
+      if (j < VD) copy_v(j);
+    }
   }
   const bool tree_ok = tree_ancestors(a, c, sm.anc, sm.up);
   cluster_wait();
   if (!tree_ok) {
     if (c.tid == 128)
-      for (int j = c.fresh; j < depth && j < c.tiles; ++j) {
+      for (int j = c.fresh; j < KD && j < c.tiles; ++j) {
         mbar_wait_own(&sm.k_full[j], 0, a.err, kErrTimeoutFull);
-        mbar_wait_own(tree_left(c, j) < kTreeTile ? &sm.tail : &sm.v_full[j], 0, a.err, kErrTimeoutFull);
+        if (j < VD) mbar_wait_own(tree_left(c, j) < kTreeTile ? &sm.tail : &sm.v_full[j], 0, a.err, kErrTimeoutFull);
       }
     return;
   }
@@ -703,10 +754,8 @@ __global__ void __launch_bounds__(kTreeTcThreads, 2) k_tree_tc(const __grid_cons
     tmem_alloc(&sm.tmem, kTreeTmemCols);
     tmem_relinquish();
   }
-  if (warp < 4) {
-    tree_rows<kTreeRows, false>(a, c, sm.anc, qs, ring);
-  }
-  if (warp == 4 && c.fresh) tree_zero_tail(ring + kTreeHalf, c.n, lane);
+  tree_rows<ROWS, 6, 4, false>(a, c, sm.anc, qs, kring, vring);
+  if (warp == 4 && c.fresh) tree_zero_tail(vring, c.n, lane);
   asm volatile("fence.proxy.async;" ::: "memory");  // queries and new rows, here or in a peer, go to MMAs
   tc_fence_before();
   if (c.share) cluster_sync_all();
@@ -717,49 +766,50 @@ __global__ void __launch_bounds__(kTreeTcThreads, 2) k_tree_tc(const __grid_cons
   float m = -INFINITY, l = 0.0f;
 
   if (warp == 4) {
+    // K runs KD - VD tiles ahead of V, whose slots are freed later
     fence_async_smem();
     bool ok = true;
-    int j = 0;
+    int j = 0, kj = KD;  // V tiles and K tiles begun
     for (; j < c.tiles; ++j) {
-      const int s = j % depth;
-      if (j >= depth) {
-        ok &= mbar_wait_own(&sm.k_empty[s], (j / depth - 1) & 1, a.err, kErrTimeoutEmpty);
-        if (!__all_sync(0xffffffffu, ok)) break;
-        if (lane == 0) copy_k(j);
-        ok &= mbar_wait_own(&sm.v_empty[s], (j / depth - 1) & 1, a.err, kErrTimeoutEmpty);
-        if (!__all_sync(0xffffffffu, ok)) {
-          mbar_wait_own(&sm.k_full[s], (j / depth) & 1, a.err, kErrTimeoutFull);
-          break;
+      if (j >= VD) {
+        if (kj < c.tiles) {
+          ok &= mbar_wait_own(&sm.k_empty[kj % KD], (kj / KD - 1) & 1, a.err, kErrTimeoutEmpty);
+          if (!__all_sync(0xffffffffu, ok)) break;
+          if (lane == 0) copy_k(kj);
+          ++kj;
         }
+        ok &= mbar_wait_own(&sm.v_empty[j % VD], (j / VD - 1) & 1, a.err, kErrTimeoutEmpty);
+        if (!__all_sync(0xffffffffu, ok)) break;
         if (lane == 0) copy_v(j);
       }
       if (j < c.fresh) {
         if (lane == 0) {
-          mbar_arrive(&sm.k_full[s]);
-          mbar_arrive(&sm.v_full[s]);
+          mbar_arrive(&sm.k_full[0]);
+          mbar_arrive(&sm.v_full[0]);
         }
       } else if (tree_left(c, j) < kTreeTile) {
         mbar_wait_own(&sm.tail, 0, a.err, kErrTimeoutFull);
-        tree_zero_tail(ring + s * kTreeStageBytes + kTreeHalf, (int)tree_left(c, j), lane);
+        tree_zero_tail(vring + (j % VD) * kTreeHalf, (int)tree_left(c, j), lane);
         fence_async_smem();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&sm.v_full[s]);
+        if (lane == 0) mbar_arrive(&sm.v_full[j % VD]);
       }
     }
     // the copies under way land before the memory is used again
-    for (int i = j > depth ? j - depth : 0; i < j; ++i) {
-      mbar_wait_own(&sm.k_full[i % depth], (i / depth) & 1, a.err, kErrTimeoutFull);
-      mbar_wait_own(&sm.v_full[i % depth], (i / depth) & 1, a.err, kErrTimeoutFull);
-    }
+    kj = min(kj, c.tiles);
+    for (int i = max(kj - KD, 0); i < kj; ++i)
+      mbar_wait_own(&sm.k_full[i % KD], (i / KD) & 1, a.err, kErrTimeoutFull);
+    for (int i = max(j - VD, 0); i < j; ++i)
+      mbar_wait_own(&sm.v_full[i % VD], (i / VD) & 1, a.err, kErrTimeoutFull);
   } else if (warp == 5) {
     // the whole warp runs the loop, so that descriptors stay in uniform registers (with one lane in
     // the loop, moving them there took 80 cycles an MMA); one lane issues
     constexpr uint32_t kIdS = idesc_f16_f32(128, kTreeTile);
     constexpr uint32_t kIdO = idesc_f16_f32(128, kHD) | (1u << 16);  // B is MN-major
-    const uint64_t qd = sw128_desc(smem_u32(qs)), kd = sw128_desc(rg), vd = tree_v_desc(rg + kTreeHalf);
+    const uint64_t qd = sw128_desc(smem_u32(qs)), kd = sw128_desc(kr), vd = tree_v_desc(vr);
     const bool leader = elect_one();
     bool ok = true;
-    int s = 0, sp = 0;            // stages of tiles j and j - 1
+    int s = 0, sp = 0;            // slots of K of tile j and of V of tile j - 1
     uint32_t ph = 0, php = 0;     // their phases
     for (int j = 0; j <= c.tiles; ++j) {
       if (j < c.tiles) {
@@ -769,10 +819,10 @@ __global__ void __launch_bounds__(kTreeTcThreads, 2) k_tree_tc(const __grid_cons
         if (!__all_sync(0xffffffffu, ok)) break;
         tc_fence_after();
         if (leader) {
-          const uint64_t kj = kd + (uint64_t)(s * (kTreeStageBytes >> 4));
+          const uint64_t kj = kd + (uint64_t)(s * (kTreeHalf >> 4));
 #pragma unroll
           for (int kk = 0; kk < 8; ++kk)
-            umma_f16(tmem + (j & 1) * 64, qd + ((kk >> 2) * (kTreeRows * 128) + (kk & 3) * 32) / 16,
+            umma_f16(tmem + (j & 1) * 64, qd + ((kk >> 2) * (ROWS * 128) + (kk & 3) * 32) / 16,
                      kj + ((kk >> 2) * (kTreeHalf / 2) + (kk & 3) * 32) / 16, kIdS, kk != 0);
           umma_commit(&sm.s_full[j & 1]);
           umma_commit(&sm.k_empty[s]);
@@ -786,7 +836,7 @@ __global__ void __launch_bounds__(kTreeTcThreads, 2) k_tree_tc(const __grid_cons
         if (!__all_sync(0xffffffffu, ok)) break;
         tc_fence_after();
         if (leader) {
-          const uint64_t vi = vd + (uint64_t)(sp * (kTreeStageBytes >> 4));
+          const uint64_t vi = vd + (uint64_t)(sp * (kTreeHalf >> 4));
 #pragma unroll
           for (int ks = 0; ks < 4; ++ks)
             umma_f16_ts(tmem + kTreeTmemO, tmem + (i & 1) * 64 + 8 * ks, vi + 2048 * ks / 16, kIdO, (i | ks) != 0);
@@ -794,9 +844,9 @@ __global__ void __launch_bounds__(kTreeTcThreads, 2) k_tree_tc(const __grid_cons
           umma_commit(&sm.v_empty[sp]);
         }
         __syncwarp();
+        if (++sp == VD) sp = 0, php ^= 1;
       }
-      sp = s, php = ph;
-      if (++s == depth) s = 0, ph ^= 1;
+      if (++s == KD) s = 0, ph ^= 1;
     }
     // nothing may be in flight when the TMEM goes
     if (c.tiles > 0) mbar_wait_own(&sm.o_done, (c.tiles - 1) & 1, a.err, kErrTimeoutFull);
@@ -879,7 +929,7 @@ __global__ void __launch_bounds__(kTreeTcThreads, 2) k_tree_tc(const __grid_cons
               c.tiles > 0 ? make_uint4(x[4 * k], x[4 * k + 1], x[4 * k + 2], x[4 * k + 3]) : make_uint4(0, 0, 0, 0);
       }
     }
-    if (row < c.R) sm.ml[row] = make_float2(m, l);
+    if (row < c.R) ml[row] = make_float2(m, l);
   }
   tc_fence_before();
   cluster_sync_all();
@@ -887,7 +937,7 @@ __global__ void __launch_bounds__(kTreeTcThreads, 2) k_tree_tc(const __grid_cons
     tc_fence_after();
     tmem_dealloc(tmem, kTreeTmemCols);
   }
-  if (warp < 4) tree_output(a, c, sm.ml, op);
+  tree_output(a, c, ml, op);
   cluster_sync_all();  // peers read this CTA's shared memory until here
 }
 
