@@ -43,30 +43,43 @@ __device__ __forceinline__ void cp_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
-// c += A . B, one m16n8k16 MMA, f16 in, f32 sums.
+// c += A . B, one m16n8k16 MMA, f16 in, f32 sums.  Not volatile: the compiler overlaps it with loads.
 __device__ __forceinline__ void mma_16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
                                           uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
       "{%8, %9}, {%0, %1, %2, %3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
+// c = A . B.
+__device__ __forceinline__ void mma_16816_zero(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                                               uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
+      "{%8, %9}, {%10, %10, %10, %10};"
+      : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
+}
+
 // One word of nibbles -> q - 8 as exact f16 pairs: (values 0, 2), (1, 3), (16, 18), (17, 19) of the
 // lane's eight.  0x6400 | n is the f16 1024 + n; a high nibble arrives as 1024 + 16 q.
+// (As C expressions, with the masks and 0x6400 as immediates, this compiled to twice the instructions.)
+__device__ __forceinline__ uint32_t and_or(uint32_t a, uint32_t mask, uint32_t bits) {
+  uint32_t d;
+  asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(d) : "r"(a), "r"(mask), "r"(bits));
+  return d;
+}
+__device__ __forceinline__ uint32_t hfma2_u32(uint32_t a, uint32_t b, uint32_t c) {
+  uint32_t d;
+  asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
+  return d;
+}
 __device__ __forceinline__ void q4_unpack(uint32_t w, uint32_t (&h)[4]) {
   const uint32_t u = w >> 8;
-  const __half2 k1032 = __half2half2(__ushort_as_half(0x6408));
-  const __half2 k16th = __half2half2(__ushort_as_half(0x2c00));
-  const __half2 km72 = __half2half2(__ushort_as_half(0xd480));
-  const uint32_t l0 = (w & 0x000f000fu) | 0x64006400u, l1 = (u & 0x000f000fu) | 0x64006400u;
-  const uint32_t h0 = (w & 0x00f000f0u) | 0x64006400u, h1 = (u & 0x00f000f0u) | 0x64006400u;
-  __half2 r[4] = {__hsub2(*(const __half2*)&l0, k1032), __hsub2(*(const __half2*)&l1, k1032),
-                  __hfma2(*(const __half2*)&h0, k16th, km72),
-                  __hfma2(*(const __half2*)&h1, k16th, km72)};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) h[i] = *(uint32_t*)&r[i];
+  h[0] = hsub2_u32(and_or(w, 0x000f000fu, 0x64006400u), 0x64086408u);               // - 1032
+  h[1] = hsub2_u32(and_or(u, 0x000f000fu, 0x64006400u), 0x64086408u);
+  h[2] = hfma2_u32(and_or(w, 0x00f000f0u, 0x64006400u), 0x2c002c00u, 0xd480d480u);  // / 16 - 72
+  h[3] = hfma2_u32(and_or(u, 0x00f000f0u, 0x64006400u), 0x2c002c00u, 0xd480d480u);
 }
 
 // x values of one block for the MMAs: (4t, 4t+2), (4t+1, 4t+3) and the same 16 higher.
@@ -79,31 +92,53 @@ __device__ __forceinline__ void q4_load_x(const uint16_t* xb, int t, uint32_t (&
   b[3] = __byte_perm(hi.x, hi.y, 0x7632);
 }
 
-// Two neighbouring blocks (36 bytes at shared address `a` of row g, `a8` of row g + 8) times NT
-// groups of 8 rows of x.
-template <int NT>
-__device__ __forceinline__ void q4_pair(uint32_t a, uint32_t a8, int t, const uint32_t (&b)[NT][2][4],
-                                        float (&acc)[NT][4]) {
+template <int OFF>
+__device__ __forceinline__ uint32_t lds32_at(uint32_t a) {
+  uint32_t v;
+  asm volatile("ld.shared.b32 %0, [%1+%2];" : "=r"(v) : "r"(a), "n"(OFF));
+  return v;
+}
+template <int OFF>
+__device__ __forceinline__ float lds_scale_at(uint32_t a) {
+  uint16_t v;
+  asm volatile("ld.shared.b16 %0, [%1+%2];" : "=h"(v) : "r"(a), "n"(OFF));
+  return h2f(v);
+}
+template <int OFF>
+__device__ __forceinline__ void lds128_at(uint32_t a, uint32_t (&v)[4]) {
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4+%5];"
+               : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3])
+               : "r"(a), "n"(OFF));
+}
+
+// The pair PAIR of neighbouring blocks (36 bytes) of row g (shared address a) and of row g + 8 (a8),
+// times NT groups of 8 rows of x.  at, a8t: the same addresses + 4 t.  Addresses differ by constants
+// from pair to pair, so a pair is 66 instructions: 12 loads, 38 to unpack, 4 MMAs, 12 to scale and add.
+template <int NT, int PAIR>
+__device__ __forceinline__ void q4_pair(uint32_t a, uint32_t a8, uint32_t at, uint32_t a8t,
+                                        const uint32_t (&b)[NT][2][4], float (&acc)[NT][4]) {
+  constexpr int O = 36 * PAIR;
   uint32_t w0[2], w1[2];  // the lane's word of blocks 0 and 1
-  w0[0] = __byte_perm(lds32(a + 4 * t), lds32(a + 4 * t + 4), 0x5432);
-  w1[0] = __byte_perm(lds32(a8 + 4 * t), lds32(a8 + 4 * t + 4), 0x5432);
-  w0[1] = lds32(a + 4 * t + 20);
-  w1[1] = lds32(a8 + 4 * t + 20);
+  w0[0] = __byte_perm(lds32_at<O>(at), lds32_at<O + 4>(at), 0x5432);
+  w1[0] = __byte_perm(lds32_at<O>(a8t), lds32_at<O + 4>(a8t), 0x5432);
+  w0[1] = lds32_at<O + 20>(at);
+  w1[1] = lds32_at<O + 20>(a8t);
+  const float d0[2] = {lds_scale_at<O>(a), lds_scale_at<O + 18>(a)};
+  const float d1[2] = {lds_scale_at<O>(a8), lds_scale_at<O + 18>(a8)};
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
-    const float d0 = h2f(lds16(a + 18 * j)), d1 = h2f(lds16(a8 + 18 * j));
     uint32_t h0[4], h1[4];
     q4_unpack(w0[j], h0);
     q4_unpack(w1[j], h1);
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-      mma_16816(c, h0[0], h1[0], h0[1], h1[1], b[n][j][0], b[n][j][1]);
+      float c[4];
+      mma_16816_zero(c, h0[0], h1[0], h0[1], h1[1], b[n][j][0], b[n][j][1]);
       mma_16816(c, h0[2], h1[2], h0[3], h1[3], b[n][j][2], b[n][j][3]);
-      acc[n][0] = __fmaf_rn(d0, c[0], acc[n][0]);
-      acc[n][1] = __fmaf_rn(d0, c[1], acc[n][1]);
-      acc[n][2] = __fmaf_rn(d1, c[2], acc[n][2]);
-      acc[n][3] = __fmaf_rn(d1, c[3], acc[n][3]);
+      acc[n][0] = __fmaf_rn(d0[j], c[0], acc[n][0]);
+      acc[n][1] = __fmaf_rn(d0[j], c[1], acc[n][1]);
+      acc[n][2] = __fmaf_rn(d1[j], c[2], acc[n][2]);
+      acc[n][3] = __fmaf_rn(d1[j], c[3], acc[n][3]);
     }
   }
 }
@@ -130,22 +165,21 @@ __global__ void __launch_bounds__(kQ4Warps * 32) k_gemv_q4(const Q4GemvArgs a) {
   const int npair = a.K / 64;
   const uint32_t wa = smem_u32(ws) + g * a.pitch, wa8 = wa + 8 * a.pitch;
   float acc[NT][4] = {};
-  uint32_t b[NT][2][4] = {};
+  uint32_t b[NT][2][4];
   auto load = [&](int p) {
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
-      if (8 * n + g < a.R) {
-        const uint16_t* xr = a.x + (int64_t)(8 * n + g) * a.K + 64 * p;
-        q4_load_x(xr, t, b[n][0]);
-        q4_load_x(xr + 32, t, b[n][1]);
-      }
+    for (int n = 0; n < NT; ++n) {
+      const uint16_t* xr = a.x + (int64_t)min(8 * n + g, a.R - 1) * a.K + 64 * p;
+      q4_load_x(xr, t, b[n][0]);
+      q4_load_x(xr + 32, t, b[n][1]);
+    }
   };
   if (warp < npair) load(warp);
   cp_wait<0>();
   __syncthreads();
   for (int p = warp; p < npair; p += kQ4Warps) {
     if (p != warp) load(p);
-    q4_pair<NT>(wa + 36 * p, wa8 + 36 * p, t, b, acc);
+    q4_pair<NT, 0>(wa + 36 * p, wa8 + 36 * p, wa + 36 * p + 4 * t, wa8 + 36 * p + 4 * t, b, acc);
   }
 #pragma unroll
   for (int n = 0; n < NT; ++n)
@@ -159,6 +193,126 @@ __global__ void __launch_bounds__(kQ4Warps * 32) k_gemv_q4(const Q4GemvArgs a) {
 #pragma unroll
     for (int k = 0; k < kQ4Warps; ++k) s = __fadd_rn(s, part[(k * 8 * NT + r) * kQ4PartPitch + n]);
     a.y[(int64_t)r * a.N + row0 + n] = f2h(s);
+  }
+}
+
+// Many rows: a persistent CTA an SM.  A group of two warps streams tiles of 16 rows through a ring of
+// its own and splits their K between them: the first warp's sum, then the second's; no barrier beyond
+// the group after x is laid out in shared memory, in the order of the B fragments ([block][8 NT rows][t],
+// 16 bytes each; rows behind R stay unset, their columns are not stored).
+//
+// A bulk copy takes the SM's copy engine about 30 cycles whatever its size (151936 x 1024 in copies of
+// 288 bytes: 37 us, of 1152: 16), so a copy is as many rows as keep the fragment loads free of bank
+// conflicts: rows are 36 K/256 words apart, so 8 / gcd(8, K/256) neighbouring rows fall into different
+// banks, and 16 bytes between the copies shift the next ones.
+constexpr int kQ4StreamGroups = 8;
+constexpr int kQ4StreamStages = 2;
+
+struct Q4StreamArgs {
+  Q4GemvArgs g;
+  int copy_rows;  // rows a copy: 1, 2, 4 or 16
+  int stage;      // bytes of a tile in shared memory
+  int ntiles;
+};
+
+__device__ __forceinline__ void bulk_g2s_plain(uint32_t dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
+      "l"(src), "r"(bytes), "r"(smem_u32(bar))
+      : "memory");
+}
+
+template <int NT>
+__global__ void __launch_bounds__(kQ4StreamGroups * 64, 1) k_gemv_q4_stream(const Q4StreamArgs s) {
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ __align__(8) uint64_t full[kQ4StreamGroups][kQ4StreamStages];
+  __shared__ __align__(8) uint64_t done[kQ4StreamGroups][kQ4StreamStages];
+  __shared__ float part[kQ4StreamGroups][kQ4StreamStages][4 * NT][32];
+  const Q4GemvArgs& a = s.g;
+  const int groups = blockDim.x >> 6, grp = threadIdx.x >> 6, half = (threadIdx.x >> 5) & 1;
+  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  uint8_t* ring = smem + grp * kQ4StreamStages * s.stage;
+  const uint32_t rg = smem_u32(ring);
+  uint4* xs = reinterpret_cast<uint4*>(smem + groups * kQ4StreamStages * s.stage);
+  const int rb = a.K / 32 * kQ4Bytes, ub = s.copy_rows * rb;  // bytes of a row, of a copy
+  // this CTA's tiles, dealt to its groups in turn
+  const int t0 = (int)((int64_t)s.ntiles * blockIdx.x / gridDim.x) + grp;
+  const int t1 = (int)((int64_t)s.ntiles * (blockIdx.x + 1) / gridDim.x);
+  auto issue = [&](int tile, int st) {  // by the first warp
+    const int rows = min(16, a.N - tile * 16), r = lane * s.copy_rows;
+    uint64_t* bar = &full[grp][st];
+    if (lane == 0) mbar_expect_tx(bar, rows * rb);
+    __syncwarp();
+    if (r < rows)
+      bulk_g2s_plain(rg + st * s.stage + lane * (ub + 16), a.w + (int64_t)(tile * 16 + r) * rb,
+                     min(s.copy_rows, rows - r) * rb, bar);
+  };
+  if (half == 0) {
+    if (lane == 0) {
+      for (int i = 0; i < kQ4StreamStages; ++i) mbar_init(&full[grp][i], 1), mbar_init(&done[grp][i], 1);
+      fence_mbar_init();
+    }
+    __syncwarp();
+    for (int i = 0; i < kQ4StreamStages; ++i)
+      if (t0 + i * groups < t1) issue(t0 + i * groups, i);
+  }
+  const int frags = a.K / 32 * a.R * 4;
+  for (int i = threadIdx.x; i < frags; i += blockDim.x) {
+    const int blk = i / (4 * a.R), n = i / 4 - blk * a.R;
+    uint32_t b[4];
+    q4_load_x(a.x + (int64_t)n * a.K + blk * 32, i & 3, b);
+    xs[(blk * 8 * NT + n) * 4 + (i & 3)] = make_uint4(b[0], b[1], b[2], b[3]);
+  }
+  __syncthreads();
+  const int g8 = g + 8, lg = __ffs(s.copy_rows) - 1;
+  const int at = (g >> lg) * (ub + 16) + (g & (s.copy_rows - 1)) * rb;
+  const int at8 = (g8 >> lg) * (ub + 16) + (g8 & (s.copy_rows - 1)) * rb;
+  const int npair = a.K / 64, p0 = half * (npair / 2), p1 = half ? npair : npair / 2;
+  int st = 0;
+  uint32_t ph = 0;
+  bool ok = true;
+  for (int tile = t0; tile < t1; tile += groups) {
+    ok &= mbar_wait_own(&full[grp][st], ph, nullptr, kErrTimeoutFull);
+    uint32_t w0 = rg + st * s.stage + at + 36 * p0, w1 = rg + st * s.stage + at8 + 36 * p0;
+    uint32_t xb = smem_u32(xs) + lane * 16 + p0 * (NT * 1024);
+    float acc[NT][4] = {};
+    for (int p = p0; p < p1; p += 2) {  // K is a multiple of 256: a warp has an even number
+      uint32_t b[2][NT][2][4];
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        if (n == 0) {
+          lds128_at<0>(xb, b[0][n][0]), lds128_at<512 * NT>(xb, b[0][n][1]);
+          lds128_at<1024 * NT>(xb, b[1][n][0]), lds128_at<1536 * NT>(xb, b[1][n][1]);
+        } else {
+          lds128_at<512>(xb, b[0][n][0]), lds128_at<512 * NT + 512>(xb, b[0][n][1]);
+          lds128_at<1024 * NT + 512>(xb, b[1][n][0]), lds128_at<1536 * NT + 512>(xb, b[1][n][1]);
+        }
+      }
+      q4_pair<NT, 0>(w0, w1, w0 + 4 * t, w1 + 4 * t, b[0], acc);
+      q4_pair<NT, 1>(w0, w1, w0 + 4 * t, w1 + 4 * t, b[1], acc);
+      w0 += 72, w1 += 72, xb += NT * 2048;
+    }
+    // the second warp runs on, up to a ring ahead: its sums go to a place per stage, and it reaches
+    // the same stage again only after a copy that the first warp has begun after reading them
+    if (half) {
+#pragma unroll
+      for (int i = 0; i < 4 * NT; ++i) part[grp][st][i][lane] = acc[i >> 2][i & 3];
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&done[grp][st]);
+    } else {
+      ok &= mbar_wait_own(&done[grp][st], ph, nullptr, kErrTimeoutFull);
+#pragma unroll
+      for (int i = 0; i < 4 * NT; ++i) acc[i >> 2][i & 3] = __fadd_rn(acc[i >> 2][i & 3], part[grp][st][i][lane]);
+      __syncwarp();  // both are done with the stage and the sums have been read
+      if (ok && tile + kQ4StreamStages * groups < t1) issue(tile + kQ4StreamStages * groups, st);
+      const int row = tile * 16 + g;
+#pragma unroll
+      for (int i = 0; i < 4 * NT; ++i) {
+        const int r = 8 * (i >> 2) + 2 * t + (i & 1), w = row + 4 * (i & 2);
+        if (r < a.R && w < a.N) a.y[(int64_t)r * a.N + w] = f2h(acc[i >> 2][i & 3]);
+      }
+    }
+    if (++st == kQ4StreamStages) st = 0, ph ^= 1;
   }
 }
 
