@@ -280,10 +280,11 @@ static int current_sms() {
 }
 
 constexpr size_t kMaxDynSmem = 200 * 1024;
+constexpr size_t kMaxOptinSmem = 226 * 1024;  // of a kernel whose static shared memory is under 1 KB
 static std::mutex g_attr_mu;
 
 template <typename F>
-static int ensure_smem_attr(F* fn, size_t bytes) {
+static int ensure_smem_attr(F* fn, size_t bytes, size_t cap = kMaxDynSmem) {
   // The dynamic shared-memory cap is a per-(kernel, device) attribute; raise it
   // once for each kernel function (keyed by its address) on each device.
   static std::set<std::pair<const void*, int>> done;
@@ -293,7 +294,7 @@ static int ensure_smem_attr(F* fn, size_t bytes) {
   std::lock_guard<std::mutex> lk(g_attr_mu);
   const auto key = std::make_pair((const void*)fn, dev);
   if (done.count(key)) return Q3_OK;
-  Q3_CUDA(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kMaxDynSmem));
+  Q3_CUDA(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)cap));
   done.insert(key);
   return Q3_OK;
 }

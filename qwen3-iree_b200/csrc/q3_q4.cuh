@@ -196,16 +196,17 @@ __global__ void __launch_bounds__(kQ4Warps * 32) k_gemv_q4(const Q4GemvArgs a) {
   }
 }
 
-// Many rows: a persistent CTA an SM.  A group of two warps streams tiles of 16 rows through a ring of
-// its own and splits their K between them: the first warp's sum, then the second's; no barrier beyond
-// the group after x is laid out in shared memory, in the order of the B fragments ([block][8 NT rows][t],
-// 16 bytes each; rows behind R stay unset, their columns are not stored).
+// Many rows: a persistent CTA an SM.  A group of KW warps streams tiles of 16 rows through a ring of
+// its own and splits their K between them; the first warp adds the others' sums to its own in order.
+// No barrier between groups after x is laid out in shared memory, in the order of the B fragments
+// ([block][8 NT rows][t], 16 bytes each; rows behind R stay unset, their columns are not stored).
 //
 // A bulk copy takes the SM's copy engine about 30 cycles whatever its size (151936 x 1024 in copies of
-// 288 bytes: 37 us, of 1152: 16), so a copy is as many rows as keep the fragment loads free of bank
+// 288 bytes: 37 us, of 1152: 25), so a copy is as many rows as keep the fragment loads free of bank
 // conflicts: rows are 36 K/256 words apart, so 8 / gcd(8, K/256) neighbouring rows fall into different
 // banks, and 16 bytes between the copies shift the next ones.
-constexpr int kQ4StreamGroups = 8;
+constexpr int kQ4StreamSplit = 2;       // KW
+constexpr int kQ4StreamMaxGroups = 10;
 constexpr int kQ4StreamStages = 2;
 
 struct Q4StreamArgs {
@@ -215,6 +216,21 @@ struct Q4StreamArgs {
   int ntiles;
 };
 
+// x fragments of two pairs of blocks.
+template <int NT>
+__device__ __forceinline__ void lds_x(uint32_t xb, uint32_t (&b)[2][NT][2][4]) {
+  lds128_at<0>(xb, b[0][0][0]);
+  lds128_at<512 * NT>(xb, b[0][0][1]);
+  lds128_at<1024 * NT>(xb, b[1][0][0]);
+  lds128_at<1536 * NT>(xb, b[1][0][1]);
+  if (NT == 2) {
+    lds128_at<512>(xb, b[0][NT - 1][0]);
+    lds128_at<512 * NT + 512>(xb, b[0][NT - 1][1]);
+    lds128_at<1024 * NT + 512>(xb, b[1][NT - 1][0]);
+    lds128_at<1536 * NT + 512>(xb, b[1][NT - 1][1]);
+  }
+}
+
 __device__ __forceinline__ void bulk_g2s_plain(uint32_t dst, const void* src, uint32_t bytes, uint64_t* bar) {
   asm volatile(
       "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
@@ -223,17 +239,19 @@ __device__ __forceinline__ void bulk_g2s_plain(uint32_t dst, const void* src, ui
 }
 
 template <int NT>
-__global__ void __launch_bounds__(kQ4StreamGroups * 64, 1) k_gemv_q4_stream(const Q4StreamArgs s) {
+__global__ void __launch_bounds__(kQ4StreamMaxGroups * kQ4StreamSplit * 32, 1) k_gemv_q4_stream(const Q4StreamArgs s) {
+  constexpr int KW = kQ4StreamSplit;
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ __align__(8) uint64_t full[kQ4StreamGroups][kQ4StreamStages];
-  __shared__ __align__(8) uint64_t done[kQ4StreamGroups][kQ4StreamStages];
-  __shared__ float part[kQ4StreamGroups][kQ4StreamStages][4 * NT][32];
+  __shared__ __align__(8) uint64_t full[kQ4StreamMaxGroups][kQ4StreamStages];
+  __shared__ __align__(8) uint64_t done[kQ4StreamMaxGroups][kQ4StreamStages];
   const Q4GemvArgs& a = s.g;
-  const int groups = blockDim.x >> 6, grp = threadIdx.x >> 6, half = (threadIdx.x >> 5) & 1;
+  const int groups = blockDim.x / (32 * KW), grp = threadIdx.x / (32 * KW), part = (threadIdx.x >> 5) % KW;
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   uint8_t* ring = smem + grp * kQ4StreamStages * s.stage;
   const uint32_t rg = smem_u32(ring);
-  uint4* xs = reinterpret_cast<uint4*>(smem + groups * kQ4StreamStages * s.stage);
+  // sums of the group's other warps, per stage: [stage][KW - 1][4 NT][32]
+  float* sums = reinterpret_cast<float*>(smem + groups * kQ4StreamStages * s.stage) + grp * kQ4StreamStages * (KW - 1) * NT * 128;
+  uint4* xs = reinterpret_cast<uint4*>(smem + groups * kQ4StreamStages * (s.stage + (KW - 1) * NT * 512));
   const int rb = a.K / 32 * kQ4Bytes, ub = s.copy_rows * rb;  // bytes of a row, of a copy
   // this CTA's tiles, dealt to its groups in turn
   const int t0 = (int)((int64_t)s.ntiles * blockIdx.x / gridDim.x) + grp;
@@ -247,9 +265,9 @@ __global__ void __launch_bounds__(kQ4StreamGroups * 64, 1) k_gemv_q4_stream(cons
       bulk_g2s_plain(rg + st * s.stage + lane * (ub + 16), a.w + (int64_t)(tile * 16 + r) * rb,
                      min(s.copy_rows, rows - r) * rb, bar);
   };
-  if (half == 0) {
+  if (part == 0) {
     if (lane == 0) {
-      for (int i = 0; i < kQ4StreamStages; ++i) mbar_init(&full[grp][i], 1), mbar_init(&done[grp][i], 1);
+      for (int i = 0; i < kQ4StreamStages; ++i) mbar_init(&full[grp][i], 1), mbar_init(&done[grp][i], KW - 1);
       fence_mbar_init();
     }
     __syncwarp();
@@ -267,7 +285,7 @@ __global__ void __launch_bounds__(kQ4StreamGroups * 64, 1) k_gemv_q4_stream(cons
   const int g8 = g + 8, lg = __ffs(s.copy_rows) - 1;
   const int at = (g >> lg) * (ub + 16) + (g & (s.copy_rows - 1)) * rb;
   const int at8 = (g8 >> lg) * (ub + 16) + (g8 & (s.copy_rows - 1)) * rb;
-  const int npair = a.K / 64, p0 = half * (npair / 2), p1 = half ? npair : npair / 2;
+  const int np = a.K / 64 / KW, p0 = part * np;  // even: K is a multiple of 256
   int st = 0;
   uint32_t ph = 0;
   bool ok = true;
@@ -276,34 +294,29 @@ __global__ void __launch_bounds__(kQ4StreamGroups * 64, 1) k_gemv_q4_stream(cons
     uint32_t w0 = rg + st * s.stage + at + 36 * p0, w1 = rg + st * s.stage + at8 + 36 * p0;
     uint32_t xb = smem_u32(xs) + lane * 16 + p0 * (NT * 1024);
     float acc[NT][4] = {};
-    for (int p = p0; p < p1; p += 2) {  // K is a multiple of 256: a warp has an even number
+    for (int p = 0; p < np; p += 2) {
       uint32_t b[2][NT][2][4];
-#pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        if (n == 0) {
-          lds128_at<0>(xb, b[0][n][0]), lds128_at<512 * NT>(xb, b[0][n][1]);
-          lds128_at<1024 * NT>(xb, b[1][n][0]), lds128_at<1536 * NT>(xb, b[1][n][1]);
-        } else {
-          lds128_at<512>(xb, b[0][n][0]), lds128_at<512 * NT + 512>(xb, b[0][n][1]);
-          lds128_at<1024 * NT + 512>(xb, b[1][n][0]), lds128_at<1536 * NT + 512>(xb, b[1][n][1]);
-        }
-      }
+      lds_x<NT>(xb, b);
       q4_pair<NT, 0>(w0, w1, w0 + 4 * t, w1 + 4 * t, b[0], acc);
       q4_pair<NT, 1>(w0, w1, w0 + 4 * t, w1 + 4 * t, b[1], acc);
       w0 += 72, w1 += 72, xb += NT * 2048;
     }
-    // the second warp runs on, up to a ring ahead: its sums go to a place per stage, and it reaches
+    // the other warps run on, up to a ring ahead: their sums go to a place per stage, and they reach
     // the same stage again only after a copy that the first warp has begun after reading them
-    if (half) {
+    float* at_sums = sums + st * (KW - 1) * NT * 128 + lane;
+    if (part) {
 #pragma unroll
-      for (int i = 0; i < 4 * NT; ++i) part[grp][st][i][lane] = acc[i >> 2][i & 3];
+      for (int i = 0; i < 4 * NT; ++i) at_sums[((part - 1) * 4 * NT + i) * 32] = acc[i >> 2][i & 3];
       __syncwarp();
       if (lane == 0) mbar_arrive(&done[grp][st]);
     } else {
       ok &= mbar_wait_own(&done[grp][st], ph, nullptr, kErrTimeoutFull);
 #pragma unroll
-      for (int i = 0; i < 4 * NT; ++i) acc[i >> 2][i & 3] = __fadd_rn(acc[i >> 2][i & 3], part[grp][st][i][lane]);
-      __syncwarp();  // both are done with the stage and the sums have been read
+      for (int k = 0; k < KW - 1; ++k)
+#pragma unroll
+        for (int i = 0; i < 4 * NT; ++i)
+          acc[i >> 2][i & 3] = __fadd_rn(acc[i >> 2][i & 3], at_sums[(k * 4 * NT + i) * 32]);
+      __syncwarp();  // all are done with the stage and the sums have been read
       if (ok && tile + kQ4StreamStages * groups < t1) issue(tile + kQ4StreamStages * groups, st);
       const int row = tile * 16 + g;
 #pragma unroll
