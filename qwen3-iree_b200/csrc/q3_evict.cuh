@@ -11,18 +11,20 @@
 // weights of one head are a few KB, from L2) and moves its share of the rows.
 //
 // Selection: keys are the weights' bits in an order-preserving form, above them all the newest.  A
-// radix select (11, 11 and 10 bits, histograms in shared memory) finds the M-th largest key and how
-// many of its ties stay; ballots then give each slot's fate and rank in slot order.
+// histogram of their top 11 bits gives the bin of the M-th largest; its keys, some tens, are ranked by
+// counting, or by two more histograms where there are many.  Ballots then give each slot's fate and its
+// rank in slot order.  28 layers of 1024 slots, 512 kept: selection 5 us, moves 7.  Small CTAs, many to
+// an SM, so that some select while others move.
 #pragma once
 
 #include "q3_common.cuh"
 
 namespace q3 {
 
-constexpr int kEvictThreads = 512;
+constexpr int kEvictThreads = 256;
 constexpr int kEvictWarps = kEvictThreads / 32;
 constexpr int kEvictBins = 2048;
-constexpr int kEvictWindow = 1024;  // moves listed in shared memory at a time
+constexpr int kEvictWindow = 512;  // moves listed in shared memory at a time, or candidates ranked
 constexpr int64_t kEvictMaxSlots = 524288;
 constexpr int kEvictKeySlots = 32768;  // up to here the keys are held in shared memory
 
@@ -47,7 +49,7 @@ struct EvictArgs {
 struct EvictSmem {
   uint32_t hist[kEvictBins];
   uint32_t warp_sum[kEvictWarps + 1];
-  uint32_t digit, above, count;
+  uint32_t digit, above, count, listed;
   int src[kEvictWindow], dst[kEvictWindow];
 };
 
@@ -91,7 +93,7 @@ __device__ __forceinline__ uint32_t evict_scan(uint32_t v, uint32_t* s, uint32_t
   return r;
 }
 
-__global__ void __launch_bounds__(kEvictThreads) k_cache_evict(const EvictArgs a) {
+__global__ void __launch_bounds__(kEvictThreads, 6) k_cache_evict(const EvictArgs a) {
   extern __shared__ __align__(128) uint8_t smem_raw[];
   EvictSmem& sm = *reinterpret_cast<EvictSmem*>(smem_raw);
   const int words_max = (int)((a.S + 31) / 32);
@@ -125,34 +127,49 @@ __global__ void __launch_bounds__(kEvictThreads) k_cache_evict(const EvictArgs a
   auto key_at = [&](int j) { return stored ? keys[j] : evict_key(w[j], sp[j], newest); };
 
   // the M-th largest key: digits of 11, 11 and 10 bits, from the top
+  constexpr int kPer = kEvictBins / kEvictThreads;
   uint32_t prefix = 0, want = (uint32_t)M, ties = 0;
 #pragma unroll 1
   for (int pass = 0; pass < 3; ++pass) {
     const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
     const uint32_t mask = pass == 2 ? 1023u : 2047u;
     for (int i = tid; i < kEvictBins; i += kEvictThreads) sm.hist[i] = 0;
+    if (tid == 0) sm.listed = 0;
     __syncthreads();
-    for (int j = tid; j < len; j += kEvictThreads) {
-      uint32_t key;
-      if (pass == 0) {
-        key = evict_key(w[j], sp[j], newest);
-        if (stored) keys[j] = key;
-      } else {
-        key = key_at(j);
-        if ((pass == 1 ? key >> 21 : key >> 10) != prefix) continue;
+    if (pass == 0) {
+      for (int j0 = tid; j0 < len; j0 += 4 * kEvictThreads) {
+        float wv[4];
+        int32_t pv[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int j = min(j0 + k * kEvictThreads, len - 1);
+          wv[k] = w[j], pv[k] = sp[j];
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int j = j0 + k * kEvictThreads;
+          if (j >= len) break;
+          const uint32_t key = evict_key(wv[k], pv[k], newest);
+          if (stored) keys[j] = key;
+          atomicAdd(&sm.hist[key >> 21], 1u);
+        }
       }
-      atomicAdd(&sm.hist[(key >> shift) & mask], 1u);
+    } else {
+      for (int j = tid; j < len; j += kEvictThreads) {
+        const uint32_t key = key_at(j);
+        if ((pass == 1 ? key >> 21 : key >> 10) == prefix) atomicAdd(&sm.hist[(key >> shift) & mask], 1u);
+      }
     }
     __syncthreads();
-    // thread i: bins 4i from the top; the bin where the count from above reaches `want`
-    const int top = kEvictBins - 1 - 4 * tid;
-    uint32_t c[4], s = 0, total;
+    // thread i: kPer bins from the top; the bin where the count from above reaches `want`
+    const int top = kEvictBins - 1 - kPer * tid;
+    uint32_t c[kPer], s = 0, total;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) c[i] = sm.hist[top - i], s += c[i];
+    for (int i = 0; i < kPer; ++i) c[i] = sm.hist[top - i], s += c[i];
     uint32_t over = evict_scan(s, sm.warp_sum, &total);
     if (over < want && want <= over + s) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
+      for (int i = 0; i < kPer; ++i) {
         if (over < want && want <= over + c[i]) sm.digit = top - i, sm.above = over, sm.count = c[i];
         over += c[i];
       }
@@ -162,6 +179,28 @@ __global__ void __launch_bounds__(kEvictThreads) k_cache_evict(const EvictArgs a
     want -= sm.above;
     ties = sm.count;
     __syncthreads();
+    if (pass == 0 && ties <= (uint32_t)kEvictWindow) {
+      // few keys in the bin: list them, and count for each the larger and the equal ones
+      uint32_t* cand = reinterpret_cast<uint32_t*>(sm.src);
+      for (int j = tid; j < len; j += kEvictThreads) {
+        const uint32_t key = key_at(j);
+        if (key >> 21 == prefix) cand[atomicAdd(&sm.listed, 1u)] = key;
+      }
+      __syncthreads();
+      const uint32_t n = ties;
+      for (uint32_t i = tid; i < n; i += kEvictThreads) {
+        const uint32_t mine = cand[i];
+        uint32_t more = 0, same = 0;
+        for (uint32_t k = 0; k < n; ++k) more += cand[k] > mine, same += cand[k] == mine;
+        if (more < want && want <= more + same) sm.digit = mine, sm.above = more, sm.count = same;  // all ties alike
+      }
+      __syncthreads();
+      prefix = sm.digit;
+      want -= sm.above;
+      ties = sm.count;
+      __syncthreads();
+      break;
+    }
   }
   const uint32_t kth = prefix;  // `want` of its `ties` slots stay
 
@@ -196,20 +235,32 @@ __global__ void __launch_bounds__(kEvictThreads) k_cache_evict(const EvictArgs a
   __syncthreads();
   const int H = (int)(total / 2);  // holes below M, and as many kept slots behind
 
-  for (int j = c0 + tid; j < c1; j += kEvictThreads)
-    if (!((bits[j >> 5] >> (j & 31)) & 1)) nw[j] = w[j], np[j] = sp[j];
+  for (int j0 = c0 + tid; j0 < c1; j0 += 4 * kEvictThreads) {
+    float wv[4];
+    int32_t pv[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int j = min(j0 + k * kEvictThreads, c1 - 1);
+      wv[k] = w[j], pv[k] = sp[j];
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int j = j0 + k * kEvictThreads;
+      if (j < c1 && !((bits[j >> 5] >> (j & 31)) & 1)) nw[j] = wv[k], np[j] = pv[k];
+    }
+  }
 
   const int m0 = (int)((int64_t)H * x / X), m1 = (int)((int64_t)H * (x + 1) / X);
   const int64_t off = b * a.seq_stride + layer * a.layer_stride + h * a.head_stride + (lane & 15) * 8;
   uint16_t* row = (lane < 16 ? a.k : a.v) + off;
   for (int r0 = m0; r0 < m1; r0 += kEvictWindow) {
     const int r1 = min(m1, r0 + kEvictWindow);
-    for (int q = tid; q < words; q += kEvictThreads) {
-      int rank = (int)pre[q];
-      for (uint32_t f = bits[q]; f; f &= f - 1, ++rank) {
-        const int j = q * 32 + __ffs(f) - 1, r = j < M ? rank : rank - H;
-        if (r >= r0 && r < r1) (j < M ? sm.dst : sm.src)[r - r0] = j;
-      }
+    for (int j = tid; j < len; j += kEvictThreads) {
+      const uint32_t f = bits[j >> 5] >> (j & 31);
+      if (!(f & 1)) continue;
+      const int rank = (int)pre[j >> 5] + __popc(bits[j >> 5] & ((1u << (j & 31)) - 1));
+      const int r = j < M ? rank : rank - H;
+      if (r >= r0 && r < r1) (j < M ? sm.dst : sm.src)[r - r0] = j;
     }
     __syncthreads();
     const int n = r1 - r0;
