@@ -512,7 +512,7 @@ typedef struct q3_kv_cache {
  * q3_decode_attention; the new K/V rows go to slots len[b] + i.
  *   qkv:      f16 [B][T][(q_heads + 2 kv_heads) * 128] raw projections
  *   n_tokens: DEVICE int32 [B], 0..T tokens (NULL: T each); rows behind them
- *             are neither read nor written, a sequence with 0 is skipped
+ *             are not used and not written, a sequence with 0 is skipped
  *   len, pos: DEVICE int64 [B]; len + n_tokens <= slots; after an eviction
  *             len < pos
  *   out:      f16 [B][T][q_heads * 128], 8-byte aligned like qkv

@@ -117,16 +117,18 @@ struct TreeCta {
   int n, R, nct, lo, tiles, fresh;  // tokens, rows, cached tiles; this CTA's first tile and tile count
   int64_t len, pos;                 // fresh: 1 in the last CTA, whose tile 0 holds the new tokens
   uint16_t *kb, *vb;
-  bool share;                       // the cluster's CTAs prepare the query rows for one another
   int parent;                       // of token `tid`
 };
 
 // Reads and checks the sequence's values; false: nothing to do (the same in all CTAs of a cluster).
-template <bool SCORED>
-__device__ __forceinline__ bool tree_begin(const TreeArgs& a, TreeCta& c) {
+__device__ __forceinline__ void tree_place(TreeCta& c) {
   c.C = gridDim.x, c.rank = blockIdx.x, c.h = blockIdx.y, c.b = blockIdx.z;
+  c.fresh = c.rank == c.C - 1;
   c.tid = threadIdx.x, c.lane = c.tid & 31;
   c.warp = __shfl_sync(0xffffffffu, c.tid >> 5, 0);  // uniform for the compiler too
+}
+template <bool SCORED>
+__device__ __forceinline__ bool tree_begin(const TreeArgs& a, TreeCta& c) {
   c.n = SCORED ? 1 : (a.n_tokens ? a.n_tokens[c.b] : a.T);
   c.len = a.len[c.b], c.pos = a.pos[c.b];
   c.parent = !SCORED && c.tid < a.T ? a.parents[(int64_t)c.b * a.T + c.tid] : -1;
@@ -140,10 +142,8 @@ __device__ __forceinline__ bool tree_begin(const TreeArgs& a, TreeCta& c) {
   const int nt = c.nct + 1;  // the new tokens count as a last tile
   c.lo = (int)((int64_t)c.rank * nt / c.C);
   c.tiles = (int)((int64_t)(c.rank + 1) * nt / c.C) - c.lo;
-  c.fresh = c.rank == c.C - 1;
   c.kb = a.k + c.b * a.seq_stride + c.h * a.head_stride;
   c.vb = a.v + c.b * a.seq_stride + c.h * a.head_stride;
-  c.share = c.C > 1 && c.R > kTreeSmallRows;  // below, pushing them costs more than preparing them
   return true;
 }
 
@@ -205,42 +205,74 @@ __device__ __forceinline__ float div_by(float v, float r, float y) {
   return y == 0.0f ? q : c;
 }
 
-// QK-RMSNorm and RoPE of the query rows into the tile `qs` (ROWS rows) of every CTA, and of the new K
-// rows, with the V rows as they are, into the first tile of the last CTA and into the cache.  The operations
+// Raw rows a warp prepares at a time: one dim of each quarter a lane, and four dims of the V row.
+template <int E>
+struct TreeRaw {
+  uint16_t x[E][4];
+  uint2 v[E];
+};
+
+// The rows to prepare are numbered over all T tokens, so that the first can be read before the number
+// of tokens is known: query rows token * group + j, then the new K rows.  SHARE: dealt out to the
+// cluster's CTAs (above 16 rows; below, pushing a row to the others costs more than preparing it).
+template <int WARPS, bool SHARE>
+struct TreeUnits {
+  int first, step, queries, units;
+  __device__ __forceinline__ TreeUnits(const TreeArgs& a, const TreeCta& c) {
+    queries = a.T << a.group_log2;
+    units = SHARE || c.fresh ? queries + a.T : queries;
+    first = SHARE ? c.rank + c.C * c.warp : c.warp;
+    step = SHARE ? WARPS * c.C : WARPS;
+  }
+};
+template <int WARPS, int E, bool SHARE>
+__device__ __forceinline__ void tree_load(const TreeArgs& a, const TreeCta& c,
+                                          const TreeUnits<WARPS, SHARE>& n, int u0, TreeRaw<E>& raw) {
+  const int gl = a.group_log2;
+  const int64_t row_el = (int64_t)(a.q_heads + 2 * a.kv_heads) * kHD;
+  const uint16_t* qkv = a.qkv + (int64_t)c.b * a.T * row_el;
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    const int u = min(u0 + e * n.step, n.units - 1);  // a repeated row is computed and dropped
+    const bool isq = u < n.queries;
+    const int tok = isq ? u >> gl : u - n.queries;
+    const uint16_t* x = qkv + tok * row_el + (isq ? (c.h << gl) + (u & ((1 << gl) - 1)) : a.q_heads + c.h) * kHD;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) raw.x[e][i] = x[c.lane + 32 * i];
+    if (!isq) raw.v[e] = *reinterpret_cast<const uint2*>(x + a.kv_heads * kHD + c.lane * 4);
+  }
+}
+
+// QK-RMSNorm and RoPE of the query rows into the tile `qs` (ROWS rows), of every CTA with SHARE (the
+// caller has waited until all CTAs run, and follows with a cluster barrier), and of the new K rows,
+// with the V rows as they are, into the first tile of the last CTA and into the cache.  The operations
 // and roundings of norm_rope_vals, a warp per row, E rows at a time without branches between them (its
-// divisions branch, and took most of 0.35 us a row).  With `share` the rows are
-// dealt out to the cluster's CTAs, which push them to one another (the caller has waited until all
-// CTAs run, and follows with a cluster barrier); otherwise each CTA prepares all it needs.
-template <int ROWS, int WARPS, int E, bool SCORED>
+// divisions branch, and took most of 0.35 us a row).  `raw`: the first rows, as tree_load read them.
+template <int ROWS, int WARPS, int E, bool SHARE, bool SCORED>
 __device__ __forceinline__ void tree_rows(const TreeArgs& a, const TreeCta& c,
+                                          const TreeUnits<WARPS, SHARE>& n, TreeRaw<E>& raw,
                                           const unsigned long long* anc, uint8_t* qs, uint8_t* knew,
                                           uint8_t* vnew) {
   const int gl = a.group_log2, lane = c.lane;
-  const int64_t row_el = (int64_t)(a.q_heads + 2 * a.kv_heads) * kHD;
-  const uint16_t* qkv = a.qkv + (int64_t)c.b * a.T * row_el;
   float gq[4], gk[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) gq[i] = h2f(a.q_norm[lane + 32 * i]), gk[i] = h2f(a.k_norm[lane + 32 * i]);
-  const int units = c.share || c.fresh ? c.R + c.n : c.R;
-  const int step = c.share ? WARPS * c.C : WARPS;
   const int last = c.C - 1;
-  for (int u0 = c.share ? c.rank + c.C * c.warp : c.warp; u0 < units; u0 += E * step) {
+  for (int u0 = n.first; u0 < n.units; u0 += E * n.step) {
     float v[E][4], cs[E][4];
     uint2 vv[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-      const int u = min(u0 + e * step, units - 1);  // a repeated row is computed and dropped
-      const bool isq = u < c.R;
-      const int tok = isq ? u >> gl : u - c.R;
-      const uint16_t* x = qkv + tok * row_el +
-                          (isq ? (c.h << gl) + (u & ((1 << gl) - 1)) : a.q_heads + c.h) * kHD;
+      const int u = min(u0 + e * n.step, n.units - 1);
+      const int tok = min(u < n.queries ? u >> gl : u - n.queries, c.n - 1);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) v[e][i] = h2f(x[lane + 32 * i]);
-      if (!isq) vv[e] = *reinterpret_cast<const uint2*>(x + a.kv_heads * kHD + lane * 4);
+      for (int i = 0; i < 4; ++i) v[e][i] = h2f(raw.x[e][i]);
+      vv[e] = raw.v[e];
       const int64_t p = (c.pos + (SCORED ? 0 : __popcll(anc[tok]) - 1)) * 64 + lane;
       cs[e][0] = a.rope_cos[p], cs[e][1] = a.rope_cos[p + 32];
       cs[e][2] = a.rope_sin[p], cs[e][3] = a.rope_sin[p + 32];
     }
+    if (u0 + E * n.step < n.units) tree_load(a, c, n, u0 + E * n.step, raw);
     float ss[E] = {};
 #pragma unroll
     for (int i = 0; i < 4; ++i)
@@ -253,7 +285,7 @@ __device__ __forceinline__ void tree_rows(const TreeArgs& a, const TreeCta& c,
     uint16_t o[E][4];
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-      const bool isq = u0 + e * step < c.R;
+      const bool isq = u0 + e * n.step < n.queries;
       const float r = __fsqrt_rn(__fadd_rn(__fmul_rn(ss[e], 0.0078125f), kEps));
       const float y = __frcp_rn(r);
       float x[4];
@@ -266,16 +298,17 @@ __device__ __forceinline__ void tree_rows(const TreeArgs& a, const TreeCta& c,
     }
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-      const int u = u0 + e * step;
-      if (u >= units) break;
-      const bool isq = u < c.R;
+      const int u = u0 + e * n.step;
+      if (u >= n.units) break;
+      const bool isq = u < n.queries;
+      if ((isq ? u >> gl : u - n.queries) >= c.n) continue;  // tokens that the sequence does not have
       if (isq) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int d = lane + 32 * i;
           *reinterpret_cast<uint16_t*>(qs + tile_at<ROWS>(u, d >> 3) + (d & 7) * 2) = o[e][i];
         }
-        if (c.share) {  // half a warp a peer
+        if (SHARE) {  // half a warp a peer
           __syncwarp();
           const uint8_t* at = qs + tile_at<ROWS>(u, lane & 15);
           const uint4 row = *reinterpret_cast<const uint4*>(at);
@@ -283,7 +316,7 @@ __device__ __forceinline__ void tree_rows(const TreeArgs& a, const TreeCta& c,
             if (p != c.rank) st_dsmem_v4(smem_u32(at), p, row);
         }
       } else {
-        const int k = u - c.R;
+        const int k = u - n.queries;
         uint16_t* kd = c.kb + (c.len + k) * a.slot_stride;
         *reinterpret_cast<uint2*>(c.vb + (c.len + k) * a.slot_stride + lane * 4) = vv[e];
         st_dsmem_v2(smem_u32(vnew) + tile_at<kTreeTile>(k, lane >> 1) + (lane & 1) * 8, last, vv[e]);
@@ -379,6 +412,10 @@ __global__ void __launch_bounds__(kTreeThreads, 3)
 
   if (threadIdx.x == 128) prefetch_tmap(&a.km), prefetch_tmap(&a.vm);
   TreeCta c;
+  tree_place(c);
+  const TreeUnits<5, false> units(a, c);
+  TreeRaw<SCORED ? 1 : 5> raw;
+  if (units.first < units.units) tree_load(a, c, units, units.first, raw);
   if (!tree_begin<SCORED>(a, c)) return;
   const int warp = c.warp, lane = c.lane, g = lane >> 2, t = lane & 3;
   const int gl = a.group_log2, G = 1 << gl;
@@ -405,10 +442,10 @@ __global__ void __launch_bounds__(kTreeThreads, 3)
   }
   const bool ok = SCORED || tree_ancestors(a, c, sm.anc, sm.up);
   cluster_wait();  // every CTA of the cluster runs
-  if (ok) tree_rows<RP, 5, SCORED ? 1 : 5, SCORED>(a, c, sm.anc, sm.q, ring, ring + kTreeHalf);
+  if (ok)
+    tree_rows<RP, 5, SCORED ? 1 : 5, false, SCORED>(a, c, units, raw, sm.anc, sm.q, ring, ring + kTreeHalf);
   if (ok && warp == 4 && c.fresh) tree_zero_tail(ring + kTreeHalf, c.n, lane);
-  if (c.share) cluster_sync_all();
-  else __syncthreads();
+  __syncthreads();
   if (!ok) {  // nothing but the first copies is under way
     if (c.tid == 128)
       for (int j = c.fresh; j < depth && j < c.tiles; ++j)
@@ -705,6 +742,10 @@ __global__ void __launch_bounds__(kTreeTcThreads, 2) k_tree_tc(const __grid_cons
 
   if (threadIdx.x == 128) prefetch_tmap(&a.km), prefetch_tmap(&a.vm);
   TreeCta c;
+  tree_place(c);
+  const TreeUnits<6, true> units(a, c);
+  TreeRaw<4> raw;
+  if (units.first < units.units) tree_load(a, c, units, units.first, raw);
   if (!tree_begin<false>(a, c)) return;
   const int gl = a.group_log2, row = c.tid, warp = c.warp, lane = c.lane;
   const uint32_t kr = smem_u32(kring), vr = smem_u32(vring);
@@ -754,11 +795,11 @@ __global__ void __launch_bounds__(kTreeTcThreads, 2) k_tree_tc(const __grid_cons
     tmem_alloc(&sm.tmem, kTreeTmemCols);
     tmem_relinquish();
   }
-  tree_rows<ROWS, 6, 4, false>(a, c, sm.anc, qs, kring, vring);
+  tree_rows<ROWS, 6, 4, true, false>(a, c, units, raw, sm.anc, qs, kring, vring);
   if (warp == 4 && c.fresh) tree_zero_tail(vring, c.n, lane);
   asm volatile("fence.proxy.async;" ::: "memory");  // queries and new rows, here or in a peer, go to MMAs
   tc_fence_before();
-  if (c.share) cluster_sync_all();
+  if (c.C > 1) cluster_sync_all();
   else __syncthreads();
   tc_fence_after();
   const uint32_t tmem = sm.tmem;
