@@ -191,6 +191,7 @@ __global__ void __launch_bounds__(kEvictThreads, 6) k_cache_evict(const EvictArg
       for (uint32_t i = tid; i < n; i += kEvictThreads) {
         const uint32_t mine = cand[i];
         uint32_t more = 0, same = 0;
+#pragma unroll 4
         for (uint32_t k = 0; k < n; ++k) more += cand[k] > mine, same += cand[k] == mine;
         if (more < want && want <= more + same) sm.digit = mine, sm.above = more, sm.count = same;  // all ties alike
       }
@@ -218,14 +219,17 @@ __global__ void __launch_bounds__(kEvictThreads, 6) k_cache_evict(const EvictArg
     tie_rank = __shfl_sync(0xffffffffu, tie_rank, 0);
   }
   uint32_t mine = 0;
+  const bool partly = want < ties;  // some of the ties go: their order counts
   for (int q = wa; q < wb; ++q) {
     const int j = q * 32 + lane;
     const uint32_t key = j < len ? key_at(j) : 0u;
-    const bool eq = j < len && key == kth;
-    const uint32_t eqs = __ballot_sync(0xffffffffu, eq);
-    const bool keep = j < len && (key > kth || (eq && tie_rank + __popc(eqs & ((1u << lane) - 1)) < want));
-    tie_rank += __popc(eqs);
-    const uint32_t sel = __ballot_sync(0xffffffffu, j < len && (j < M ? !keep : keep));
+    bool keep = key >= kth;
+    if (partly) {
+      const uint32_t eqs = __ballot_sync(0xffffffffu, j < len && key == kth);
+      keep = key > kth || (key == kth && tie_rank + __popc(eqs & ((1u << lane) - 1)) < want);
+      tie_rank += __popc(eqs);
+    }
+    const uint32_t sel = __ballot_sync(0xffffffffu, j < len && (j < M) != keep);
     if (lane == 0) bits[q] = sel, pre[q] = mine;
     mine += __popc(sel);
   }
