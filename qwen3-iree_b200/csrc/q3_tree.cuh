@@ -102,6 +102,10 @@ __device__ __forceinline__ void st_dsmem_v2(uint32_t local_addr, uint32_t rank, 
                : "memory");
 }
 
+__device__ __forceinline__ void st_dsmem_u8(uint32_t local_addr, uint32_t rank, uint32_t v) {
+  asm volatile("st.shared::cluster.b8 [%0], %1;" ::"r"(dsmem_map(local_addr, rank)), "r"(v) : "memory");
+}
+
 // Byte offset of 16-byte chunk c (0..15) of row r in a tile of ROWS 256-byte rows: two halves of 64
 // dims, each in the SWIZZLE_128B layout (128-byte rows, the chunk xored with the row).  The 8 rows of
 // an ldmatrix fall into different banks, and the tensor core reads it K-major (rows along N) or
@@ -205,6 +209,14 @@ __device__ __forceinline__ float div_by(float v, float r, float y) {
   return y == 0.0f ? q : c;
 }
 
+// Two f16 with zeros for infinities and NaNs.
+__device__ __forceinline__ uint32_t finite_h2(uint32_t h) {
+  uint32_t m = 0;
+  if ((h & 0x00007c00u) != 0x00007c00u) m |= 0x0000ffffu;
+  if ((h & 0x7c000000u) != 0x7c000000u) m |= 0xffff0000u;
+  return h & m;
+}
+
 // Raw rows a warp prepares at a time: one dim of each quarter a lane, and four dims of the V row.
 template <int E>
 struct TreeRaw {
@@ -248,11 +260,14 @@ __device__ __forceinline__ void tree_load(const TreeArgs& a, const TreeCta& c,
 // with the V rows as they are, into the first tile of the last CTA and into the cache.  The operations
 // and roundings of norm_rope_vals, a warp per row, E rows at a time without branches between them (its
 // divisions branch, and took most of 0.35 us a row).  `raw`: the first rows, as tree_load read them.
+// An infinity or NaN of a V row must not reach the tokens that do not see it (0 * inf is a NaN), so the
+// tile gets zeros for them, and odd[k] says that token k has some: tree_add_odd gives them to those that
+// do see them.
 template <int ROWS, int WARPS, int E, bool SHARE, bool SCORED>
 __device__ __forceinline__ void tree_rows(const TreeArgs& a, const TreeCta& c,
                                           const TreeUnits<WARPS, SHARE>& n, TreeRaw<E>& raw,
                                           const unsigned long long* anc, uint8_t* qs, uint8_t* knew,
-                                          uint8_t* vnew) {
+                                          uint8_t* vnew, uint8_t* odd) {
   const int gl = a.group_log2, lane = c.lane;
   float gq[4], gk[4];
 #pragma unroll
@@ -319,7 +334,11 @@ __device__ __forceinline__ void tree_rows(const TreeArgs& a, const TreeCta& c,
         const int k = u - n.queries;
         uint16_t* kd = c.kb + (c.len + k) * a.slot_stride;
         *reinterpret_cast<uint2*>(c.vb + (c.len + k) * a.slot_stride + lane * 4) = vv[e];
-        st_dsmem_v2(smem_u32(vnew) + tile_at<kTreeTile>(k, lane >> 1) + (lane & 1) * 8, last, vv[e]);
+        uint2 fin = make_uint2(finite_h2(vv[e].x), finite_h2(vv[e].y));
+        const bool any = __any_sync(0xffffffffu, fin.x != vv[e].x || fin.y != vv[e].y);
+        if (SCORED) fin = vv[e];  // one token, which sees itself
+        else if (lane == 0) st_dsmem_u8(smem_u32(odd + k), last, any);
+        st_dsmem_v2(smem_u32(vnew) + tile_at<kTreeTile>(k, lane >> 1) + (lane & 1) * 8, last, fin);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int d = lane + 32 * i;
@@ -336,6 +355,24 @@ __device__ __forceinline__ void tree_rows(const TreeArgs& a, const TreeCta& c,
 __device__ __forceinline__ void tree_zero_tail(uint8_t* v, int nv, int lane) {
   for (int i = nv * 16 + lane; i < kTreeTile * 16; i += 32)
     *reinterpret_cast<uint4*>(v + tile_at<kTreeTile>(i >> 4, i & 15)) = make_uint4(0u, 0u, 0u, 0u);
+}
+
+// Tokens whose V rows hold infinities or NaNs (by a whole warp).
+__device__ __forceinline__ unsigned long long tree_odd(const TreeCta& c, const uint8_t* odd) {
+  const uint32_t lo = __ballot_sync(0xffffffffu, c.lane < c.n && odd[c.lane]);
+  const uint32_t hi = __ballot_sync(0xffffffffu, c.lane + 32 < c.n && odd[c.lane + 32]);
+  return (unsigned long long)hi << 32 | lo;
+}
+// Adds dim d's infinities and NaNs of the tokens in `from` to x.
+__device__ __forceinline__ float tree_add_odd(const TreeArgs& a, const TreeCta& c, unsigned long long from, int d,
+                                              float x) {
+  const int64_t row_el = (int64_t)(a.q_heads + 2 * a.kv_heads) * kHD;
+  const uint16_t* v = a.qkv + (int64_t)c.b * a.T * row_el + (int64_t)(a.q_heads + a.kv_heads + c.h) * kHD + d;
+  for (; from; from &= from - 1) {
+    const uint16_t h = v[(__ffsll((long long)from) - 1) * row_el];
+    if ((h & 0x7c00u) == 0x7c00u) x = __fadd_rn(x, h2f(h));
+  }
+  return x;
 }
 
 // Keys of tile j that row `row` sees, as bits; `nv`: keys the tile holds.
@@ -395,6 +432,7 @@ struct TreeSmallSmem {  // behind the ring
   float2 ml[kTreeSmallRows];      // this CTA's
   unsigned long long anc[kTreeMaxTokens];
   int up[kTreeMaxTokens];
+  uint8_t odd[kTreeMaxTokens];
   uint64_t full[kTreeMaxDepth], empty[kTreeMaxDepth], tail;
 };
 constexpr size_t tree_small_bytes(int depth) {
@@ -443,7 +481,8 @@ __global__ void __launch_bounds__(kTreeThreads, 3)
   const bool ok = SCORED || tree_ancestors(a, c, sm.anc, sm.up);
   cluster_wait();  // every CTA of the cluster runs
   if (ok)
-    tree_rows<RP, 5, SCORED ? 1 : 5, false, SCORED>(a, c, units, raw, sm.anc, sm.q, ring, ring + kTreeHalf);
+    tree_rows<RP, 5, SCORED ? 1 : 5, false, SCORED>(a, c, units, raw, sm.anc, sm.q, ring, ring + kTreeHalf,
+                                                         sm.odd);
   if (ok && warp == 4 && c.fresh) tree_zero_tail(ring + kTreeHalf, c.n, lane);
   __syncthreads();
   if (!ok) {  // nothing but the first copies is under way
@@ -453,8 +492,10 @@ __global__ void __launch_bounds__(kTreeThreads, 3)
     return;
   }
 
+  const unsigned long long odd = !SCORED && c.fresh ? tree_odd(c, sm.odd) : 0ull;
   float o[16][4] = {}, m[2] = {-INFINITY, -INFINITY}, l[2] = {};
   if (warp == 4) {
+    fence_async_smem();  // the new tokens' stage was written by threads, later by copies
     bool run = true;
     int j = 0;
     for (; j < c.tiles; ++j) {
@@ -477,98 +518,98 @@ __global__ void __launch_bounds__(kTreeThreads, 3)
     for (int i = j > depth ? j - depth : 0; i < j; ++i)
       mbar_wait_own(&sm.full[i % depth], (i / depth) & 1, a.err, kErrTimeoutFull);
   } else {
-  uint32_t qf[8][4];
+    uint32_t qf[8][4];
 #pragma unroll
-  for (int kk = 0; kk < 8; ++kk)
-    ldsm4(qf[kk], smem_u32(sm.q) + tile_at<RP>((lane & 7) + ((lane >> 3) & 1) * 8, 2 * kk + (lane >> 4)));
+    for (int kk = 0; kk < 8; ++kk)
+      ldsm4(qf[kk], smem_u32(sm.q) + tile_at<RP>((lane & 7) + ((lane >> 3) & 1) * 8, 2 * kk + (lane >> 4)));
 
-  bool run = true;
-  for (int j = 0; j < c.tiles; ++j) {
-    const int sl = j % depth;
-    const uint32_t st = rg + sl * kTreeStageBytes;
-    const bool fresh = j < c.fresh;
-    const int64_t left = tree_left(c, j);
-    const int nv = fresh ? c.n : (int)(left < kTreeTile ? left : kTreeTile);
-    run &= mbar_wait_own(&sm.full[sl], (j / depth) & 1, a.err, kErrTimeoutFull);
-    if (!__all_sync(0xffffffffu, run)) break;
-    const int k0 = warp * 16;
-    if (k0 < nv) {
-    float s[2][4] = {};
+    bool run = true;
+    for (int j = 0; j < c.tiles; ++j) {
+      const int sl = j % depth;
+      const uint32_t st = rg + sl * kTreeStageBytes;
+      const bool fresh = j < c.fresh;
+      const int64_t left = tree_left(c, j);
+      const int nv = fresh ? c.n : (int)(left < kTreeTile ? left : kTreeTile);
+      run &= mbar_wait_own(&sm.full[sl], (j / depth) & 1, a.err, kErrTimeoutFull);
+      if (!__all_sync(0xffffffffu, run)) break;
+      const int k0 = warp * 16;
+      if (k0 < nv) {
+        float s[2][4] = {};
 #pragma unroll
-    for (int kk = 0; kk < 8; ++kk) {
-      uint32_t bf[4];
-      ldsm4(bf, st + tile_at<kTreeTile>(k0 + (lane & 7) + (lane >> 4) * 8, 2 * kk + ((lane >> 3) & 1)));
-      mma_16816(s[0], qf[kk][0], qf[kk][1], qf[kk][2], qf[kk][3], bf[0], bf[1]);
-      mma_16816(s[1], qf[kk][0], qf[kk][1], qf[kk][2], qf[kk][3], bf[2], bf[3]);
-    }
-    if (fresh || nv < kTreeTile) {
+        for (int kk = 0; kk < 8; ++kk) {
+          uint32_t bf[4];
+          ldsm4(bf, st + tile_at<kTreeTile>(k0 + (lane & 7) + (lane >> 4) * 8, 2 * kk + ((lane >> 3) & 1)));
+          mma_16816(s[0], qf[kk][0], qf[kk][1], qf[kk][2], qf[kk][3], bf[0], bf[1]);
+          mma_16816(s[1], qf[kk][0], qf[kk][1], qf[kk][2], qf[kk][3], bf[2], bf[3]);
+        }
+        if (fresh || nv < kTreeTile) {
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const unsigned long long see = tree_seen(c, sm.anc, fresh && !SCORED, g + 8 * e, nv, gl);
+          for (int e = 0; e < 2; ++e) {
+            const unsigned long long see = tree_seen(c, sm.anc, fresh && !SCORED, g + 8 * e, nv, gl);
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (!((see >> (k0 + 8 * (i >> 1) + 2 * t + (i & 1))) & 1)) s[i >> 1][2 * e + (i & 1)] = -INFINITY;
+            for (int i = 0; i < 4; ++i)
+              if (!((see >> (k0 + 8 * (i >> 1) + 2 * t + (i & 1))) & 1)) s[i >> 1][2 * e + (i & 1)] = -INFINITY;
+          }
+        }
+        if (SCORED && g < G) {
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+            *reinterpret_cast<float2*>(score + g * a.score_cap + j * kTreeTile + k0 + 8 * i + 2 * t) =
+                make_float2(s[i][0], s[i][1]);
+        }
+        uint32_t pf[2][2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float mx = fmaxf(fmaxf(s[0][2 * e], s[0][2 * e + 1]), fmaxf(s[1][2 * e], s[1][2 * e + 1]));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+          const float mn = fmaxf(m[e], __fmul_rn(mx, kTreeLog2Scale));
+          const float mu = mn == -INFINITY ? 0.0f : mn;  // a row that sees no key yet
+          const float al = ex2(__fsub_rn(m[e], mu));
+          m[e] = mn;
+          float sum = 0.0f;
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const float p0 = ex2(__fmaf_rn(s[i][2 * e], kTreeLog2Scale, -mu));
+            const float p1 = ex2(__fmaf_rn(s[i][2 * e + 1], kTreeLog2Scale, -mu));
+            sum = __fadd_rn(sum, __fadd_rn(p0, p1));
+            pf[i][e] = pack_h2(p0, p1);
+          }
+          l[e] = __fmaf_rn(l[e], al, sum);
+#pragma unroll
+          for (int d = 0; d < 16; ++d) {
+            o[d][2 * e] = __fmul_rn(o[d][2 * e], al);
+            o[d][2 * e + 1] = __fmul_rn(o[d][2 * e + 1], al);
+          }
+        }
+#pragma unroll
+        for (int d = 0; d < 8; ++d) {
+          uint32_t bf[4];
+          ldsm4_t(bf, st + kTreeHalf +
+                          tile_at<kTreeTile>(k0 + (lane & 7) + ((lane >> 3) & 1) * 8, 2 * d + (lane >> 4)));
+          mma_16816(o[2 * d], pf[0][0], pf[0][1], pf[1][0], pf[1][1], bf[0], bf[1]);
+          mma_16816(o[2 * d + 1], pf[0][0], pf[0][1], pf[1][0], pf[1][1], bf[2], bf[3]);
+        }
       }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sm.empty[sl]);
     }
-    if (SCORED && g < G) {
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-        *reinterpret_cast<float2*>(score + g * a.score_cap + j * kTreeTile + k0 + 8 * i + 2 * t) =
-            make_float2(s[i][0], s[i][1]);
-    }
-    uint32_t pf[2][2];
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      float mx = fmaxf(fmaxf(s[0][2 * e], s[0][2 * e + 1]), fmaxf(s[1][2 * e], s[1][2 * e + 1]));
-      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-      const float mn = fmaxf(m[e], __fmul_rn(mx, kTreeLog2Scale));
-      const float mu = mn == -INFINITY ? 0.0f : mn;  // a row that sees no key yet
-      const float al = ex2(__fsub_rn(m[e], mu));
-      m[e] = mn;
-      float sum = 0.0f;
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const float p0 = ex2(__fmaf_rn(s[i][2 * e], kTreeLog2Scale, -mu));
-        const float p1 = ex2(__fmaf_rn(s[i][2 * e + 1], kTreeLog2Scale, -mu));
-        sum = __fadd_rn(sum, __fadd_rn(p0, p1));
-        pf[i][e] = pack_h2(p0, p1);
-      }
-      l[e] = __fmaf_rn(l[e], al, sum);
-#pragma unroll
-      for (int d = 0; d < 16; ++d) {
-        o[d][2 * e] = __fmul_rn(o[d][2 * e], al);
-        o[d][2 * e + 1] = __fmul_rn(o[d][2 * e + 1], al);
-      }
-    }
-#pragma unroll
-    for (int d = 0; d < 8; ++d) {
-      uint32_t bf[4];
-      ldsm4_t(bf, st + kTreeHalf +
-                      tile_at<kTreeTile>(k0 + (lane & 7) + ((lane >> 3) & 1) * 8, 2 * d + (lane >> 4)));
-      mma_16816(o[2 * d], pf[0][0], pf[0][1], pf[1][0], pf[1][1], bf[0], bf[1]);
-      mma_16816(o[2 * d + 1], pf[0][0], pf[0][1], pf[1][0], pf[1][1], bf[2], bf[3]);
-    }
-    }
-    __syncwarp();
-    if (lane == 0) mbar_arrive(&sm.empty[sl]);
-  }
   }
   __syncthreads();  // the ring becomes the partial outputs
 
   if (warp < 4) {
 #pragma unroll
-  for (int e = 0; e < 2; ++e) {
-    const int row = g + 8 * e;
-    float s = l[e];
-    s = __fadd_rn(s, __shfl_xor_sync(0xffffffffu, s, 1));
-    s = __fadd_rn(s, __shfl_xor_sync(0xffffffffu, s, 2));
-    if (t == 0) sm.mlw[warp][row] = make_float2(m[e], s);
+    for (int e = 0; e < 2; ++e) {
+      const int row = g + 8 * e;
+      float s = l[e];
+      s = __fadd_rn(s, __shfl_xor_sync(0xffffffffu, s, 1));
+      s = __fadd_rn(s, __shfl_xor_sync(0xffffffffu, s, 2));
+      if (t == 0) sm.mlw[warp][row] = make_float2(m[e], s);
 #pragma unroll
-    for (int d = 0; d < 16; ++d)
-      *reinterpret_cast<float2*>(op + (warp * RP + row) * kTreeOPitch + 8 * d + 2 * t) =
-          make_float2(o[d][2 * e], o[d][2 * e + 1]);
-  }
+      for (int d = 0; d < 16; ++d)
+        *reinterpret_cast<float2*>(op + (warp * RP + row) * kTreeOPitch + 8 * d + 2 * t) =
+            make_float2(o[d][2 * e], o[d][2 * e + 1]);
+    }
   }
   __syncthreads();
   // the warps' partials into one per row: a warp a row, four dims a lane
@@ -586,6 +627,11 @@ __global__ void __launch_bounds__(kTreeThreads, 3)
       L = __fmaf_rn(q.y, f, L);
       s.x = __fmaf_rn(x.x, f, s.x), s.y = __fmaf_rn(x.y, f, s.y);
       s.z = __fmaf_rn(x.z, f, s.z), s.w = __fmaf_rn(x.w, f, s.w);
+    }
+    if (odd) {
+      const unsigned long long from = odd & sm.anc[r >> gl];
+      s.x = tree_add_odd(a, c, from, 4 * lane, s.x), s.y = tree_add_odd(a, c, from, 4 * lane + 1, s.y);
+      s.z = tree_add_odd(a, c, from, 4 * lane + 2, s.z), s.w = tree_add_odd(a, c, from, 4 * lane + 3, s.w);
     }
     *reinterpret_cast<float4*>(op + r * kTreeOPitch + 4 * lane) = s;
     if (lane == 0) sm.ml[r] = make_float2(M, L);
@@ -706,6 +752,7 @@ struct TreeTc {
 struct TreeTcSmem {  // behind the ring
   unsigned long long anc[kTreeMaxTokens];
   int up[kTreeMaxTokens];
+  uint8_t odd[kTreeMaxTokens];
   uint64_t k_full[kTreeMaxSlots], k_empty[kTreeMaxSlots], v_full[kTreeMaxSlots], v_empty[kTreeMaxSlots];
   uint64_t s_full[2], p_full[2], o_done, tail;
   uint32_t tmem;
@@ -795,7 +842,7 @@ __global__ void __launch_bounds__(kTreeTcThreads, 2) k_tree_tc(const __grid_cons
     tmem_alloc(&sm.tmem, kTreeTmemCols);
     tmem_relinquish();
   }
-  tree_rows<ROWS, 6, 4, true, false>(a, c, units, raw, sm.anc, qs, kring, vring);
+  tree_rows<ROWS, 6, 4, true, false>(a, c, units, raw, sm.anc, qs, kring, vring, sm.odd);
   if (warp == 4 && c.fresh) tree_zero_tail(vring, c.n, lane);
   asm volatile("fence.proxy.async;" ::: "memory");  // queries and new rows, here or in a peer, go to MMAs
   tc_fence_before();
@@ -970,7 +1017,13 @@ __global__ void __launch_bounds__(kTreeTcThreads, 2) k_tree_tc(const __grid_cons
               c.tiles > 0 ? make_uint4(x[4 * k], x[4 * k + 1], x[4 * k + 2], x[4 * k + 3]) : make_uint4(0, 0, 0, 0);
       }
     }
-    if (row < c.R) ml[row] = make_float2(m, l);
+    const unsigned long long odd = c.fresh ? tree_odd(c, sm.odd) : 0ull;
+    if (row < c.R) {
+      if (odd & sm.anc[row >> gl])
+        for (int d = 0; d < kHD; ++d)
+          op[row * kTreeOPitch + d] = tree_add_odd(a, c, odd & sm.anc[row >> gl], d, op[row * kTreeOPitch + d]);
+      ml[row] = make_float2(m, l);
+    }
   }
   tc_fence_before();
   cluster_sync_all();

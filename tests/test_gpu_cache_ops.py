@@ -213,6 +213,89 @@ def test_tree_attention_huge_scores(gpu):
     assert np.isfinite(out).all()
 
 
+@pytest.mark.parametrize("T", [6, 30, 60])
+def test_tree_attention_odd_values_stay_on_their_branch(gpu, T):
+    """An infinity and a NaN in a drafted token's V row reach the tokens that see it, in their dims, and
+    no other; a token whose Q and K are NaN spoils only its descendants."""
+    t = Tree(gpu, 30 + T, T, [130], kind="mixed")
+    clean = t.upload().call().check()
+    par = t.parents[0]
+    sees = lambda i, j: i == j or (par[i] >= 0 and sees(par[i], j))
+    bad, lost = T // 3, T - 2
+    par[lost] = -1                                        # apart from the first
+    par[bad] = -1
+    base = t.upload().call().check()
+    x = t.qkv[0].reshape(T, 32, HD)
+    x[bad, 24:, 3], x[bad, 24:, 90] = -np.inf, np.nan     # V of every kv head
+    x[lost, :24] = np.nan                                 # its Q and K
+    t.upload().call()
+    got, k = t.out.download()[0].reshape(T, 16, HD), t.c.download()[0]
+    want = base[0].reshape(T, 16, HD)
+    for i in range(T):
+        dims = np.ones(HD, bool)
+        if sees(i, lost):
+            assert np.isnan(got[i]).all()
+            continue
+        if sees(i, bad):
+            dims[[3, 90]] = False
+            assert (got[i, :, 3] == -np.inf).all() and np.isnan(got[i, :, 90]).all()
+        assert np.array_equal(bits(got[i][:, dims]), bits(want[i][:, dims])), i
+    v = t.c.view(t.c.download()[1])[0, 0, :, 130 + bad]
+    assert (v[:, 3] == -np.inf).all() and np.isnan(v[:, 90]).all()  # the cache holds them as they are
+    assert clean.shape == base.shape
+
+
+def test_first_calls_inside_a_capture(gpu):
+    """A process whose first call of each operator is captured: set-up is legal there, and the replay
+    gives what eager calls give."""
+    import subprocess
+    import sys
+
+    code = """
+import sys, ctypes
+sys.path[:0] = %r
+import numpy as np, q3b200 as q3
+from cache_reference import *
+q3.set_device(0)
+rng = np.random.default_rng(5)
+c = Cache(rng, 1, 1, 200).upload(q3)
+cos, sin = (up(q3, x) for x in rope_tables(q3, 256))
+g = up(q3, np.ones(HD, np.float16))
+n, zero = 40, up(q3, np.zeros(1, np.int32))
+qkv = up(q3, rng.standard_normal((n, 4096)).astype(np.float16))
+par = up(q3, (np.arange(n) - 1).astype(np.int32))
+lens, new_len, newer = (up(q3, np.array([x])) for x in (100, 0, 0))
+acc = up(q3, np.arange(1, n, 2).astype(np.int32)); nacc = up(q3, np.array([20], np.int32))
+w, w2 = (up(q3, np.ones((1, 1, 8, 200), np.float32)) for _ in range(2))
+sp, sp2 = (up(q3, np.tile(np.arange(200, dtype=np.int32), (1, 1, 8, 1))) for _ in range(2))
+blocks = up(q3, q4_blocks(rng, 4096, 256)); many = up(q3, q4_blocks(rng, 20000, 256))
+x = up(q3, rng.standard_normal((2, 256)).astype(np.float16))
+ys = [q3.DeviceArray((2, m), np.float16) for m in (4096, 20000)]
+outs = [q3.DeviceArray((n, 2048), np.float16, zero=True) for _ in range(3)]
+def step(st):
+    q3.call("q3_gemv_q4", blocks.ptr, x.ptr, ys[0].ptr, 4096, 256, 2, st)
+    q3.call("q3_gemv_q4", many.ptr, x.ptr, ys[1].ptr, 20000, 256, 2, st)
+    for T, o in ((n, outs[0]), (8, outs[1])):
+        q3.call("q3_tree_attention", qkv.ptr, g.ptr, g.ptr, cos.ptr, sin.ptr, 256, c.kv, 0, 1, T, par.ptr, None, lens.ptr, lens.ptr, o.ptr, zero.ptr, st)
+    q3.call("q3_tree_commit", c.kv, 0, 1, 1, 20, acc.ptr, nacc.ptr, lens.ptr, new_len.ptr, lens.ptr, w.ptr, sp.ptr, zero.ptr, st)
+    q3.call("q3_decode_attention_scored", qkv.ptr, g.ptr, g.ptr, cos.ptr, sin.ptr, 256, c.kv, 0, 1, new_len.ptr, new_len.ptr, w.ptr, w2.ptr, sp.ptr, outs[2].ptr, zero.ptr, st)
+    q3.call("q3_cache_evict", c.kv, 0, 1, 1, 64, 8, new_len.ptr, new_len.ptr, w2.ptr, sp.ptr, newer.ptr, w.ptr, sp2.ptr, zero.ptr, st)
+st, ex = ctypes.c_void_p(), ctypes.c_void_p()
+q3.call("q3_stream_create", ctypes.byref(st))
+q3.call("q3_graph_capture_begin", st); step(st); q3.call("q3_graph_capture_end", st, ctypes.byref(ex))
+def run(f):
+    c.dk.upload(c.k); c.dv.upload(c.v); w.upload(np.ones((1, 1, 8, 200), np.float32))
+    f(); q3.call("q3_stream_synchronize", st)
+    return [a.download().tobytes() for a in (*ys, *outs, w2, sp2, newer, c.dk, c.dv, zero)]
+a = run(lambda: q3.call("q3_graph_launch", ex, st)); b = run(lambda: step(st))
+assert a == b and zero.download()[0] == 0 and newer.download()[0] == 64
+q3.call("q3_graph_destroy", ex)
+print("same")
+""" % [p for p in sys.path if p.endswith(("qwen3-iree_b200", "tests"))]
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=120)
+    assert r.returncode == 0 and "same" in r.stdout, r.stderr[-2000:]
+
+
 def test_tree_attention_beyond_4_gb(gpu):
     """The second sequence's rows lie more than 2^32 bytes (and 2^31 elements) behind the first's."""
     t = Tree(gpu, 12, 3, [70, 90], S=128)
