@@ -20,6 +20,7 @@ token-id lists -- seeded ones by default, one line of ids per prompt with
   python -m q3b200.benchmark --num-prompts 1 --prompt-len 1 --max-tokens 3 --no-warmup
       (the smallest whole decode: 4 steps of 141 launches, for profilers)
   python -m q3b200.benchmark --gemv-stream gate_up   (GEMV HBM GB/s, 28 layers a launch)
+  python -m q3b200.benchmark --cache-op tree --tokens 64 --context 0 32000   (drafted-token operators)
 """
 from __future__ import annotations
 
@@ -154,6 +155,85 @@ def gemv_stream(dw, name: str, reps: int = 20, warmup: int = 3) -> dict:
     us = total_ms * 1e3 / reps
     b = 28 * (bpl + 2 * K + 2 * N)
     return {"us_per_launch": us, "bytes": b, "gbs": b / (us * 1e-6) / 1e9, "l2": "flushed"}
+
+
+CACHE_OPS = ("q4", "tree", "scored", "evict")
+
+
+def _random_f16(n: int, seed: int):
+    """n f16 values on the device, N(0, 1), a block of 2^22 repeated."""
+    from . import DeviceArray
+    from ._lib import call
+
+    d = DeviceArray((n,), np.float16)
+    block = DeviceArray.from_host(np.random.default_rng(seed).standard_normal(1 << 22).astype(np.float16))
+    for at in range(0, n, 1 << 22):
+        call("q3_memcpy_dtod", d.ptr + 2 * at, block.ptr, 2 * min(1 << 22, n - at), None)
+    call("q3_stream_synchronize", None)
+    return d
+
+
+def cache_op(name: str, B: int, length: int, tokens: int, reps: int = 20, warmup: int = 3) -> dict:
+    """One of the drafted-token operators on random data, L2 flushed before every timed call:
+    q4: the vocabulary matrix as Q4_0 times `tokens` rows; tree: `tokens` drafted tokens (a chain)
+    over `length` cached slots, one layer, B sequences; scored: one token; evict: 28 layers of
+    `length` slots down to three quarters."""
+    from . import DeviceArray, Events, KVCache
+    from ._lib import call
+    from .weights import HD, LAYERS, NKV, NQ, VOCAB
+
+    rng = np.random.default_rng(0)
+    up = lambda a: DeviceArray.from_host(np.ascontiguousarray(a))
+    err = up(np.zeros(1, np.int32))
+    layers = LAYERS if name == "evict" else 1
+    S = length + (0 if name == "evict" else tokens)
+    if name == "q4":
+        N, K = VOCAB, 1024
+        w = up(np.resize(rng.integers(0, 60, 1 << 20, dtype=np.uint8), N * K // 32 * 18))
+        x, y = up(rng.standard_normal((tokens, K)).astype(np.float16)), DeviceArray((tokens, N), np.float16)
+        run = lambda: call("q3_gemv_q4", w.ptr, x.ptr, y.ptr, N, K, tokens, None)
+        moved = N * K // 32 * 18 + 2 * tokens * (N + K)
+    else:
+        k, v = (_random_f16(B * layers * S * NKV * HD, i) for i in (1, 2))
+        kv = KVCache(k.ptr, v.ptr, layers * S * NKV * HD, S * NKV * HD, NKV * HD, HD, S, layers, NQ, NKV)
+        lens = up(np.full(B, length, np.int64))
+        shape = (B, layers, NKV, S)
+        weight = up(rng.random(shape, np.float32))
+        slot_pos = up(np.broadcast_to(np.arange(S, dtype=np.int32), shape))
+    if name in ("tree", "scored"):
+        T = tokens if name == "tree" else 1
+        qkv = _random_f16(B * T * (NQ + 2 * NKV) * HD, 3)
+        ones = up(np.ones(HD, np.float16))
+        cos, sin = np.empty((S, 64), np.float32), np.empty((S, 64), np.float32)
+        call("q3_rope_table", S, cos.ctypes.data, sin.ctypes.data)
+        cos, sin, out = up(cos), up(sin), DeviceArray((B, T, NQ * HD), np.float16)
+        parents = up(np.tile(np.arange(T, dtype=np.int32) - 1, (B, 1)))
+        head = (qkv.ptr, ones.ptr, ones.ptr, cos.ptr, sin.ptr, S, kv, 0, B)
+        if name == "tree":
+            run = lambda: call("q3_tree_attention", *head, T, parents.ptr, None, lens.ptr, lens.ptr, out.ptr,
+                               err.ptr, None)
+        else:
+            run = lambda: call("q3_decode_attention_scored", *head, lens.ptr, lens.ptr, weight.ptr, weight.ptr,
+                               slot_pos.ptr, out.ptr, err.ptr, None)
+        moved = B * length * NKV * (512 + (8 if name == "scored" else 0))
+    elif name == "evict":
+        budget = max(1, length * 3 // 4)
+        new_len, new_w, new_p = DeviceArray((B,), np.int64), DeviceArray(shape, np.float32), DeviceArray(shape, np.int32)
+        run = lambda: call("q3_cache_evict", kv, 0, layers, B, budget, min(64, budget), lens.ptr, lens.ptr, weight.ptr,
+                           slot_pos.ptr, new_len.ptr, new_w.ptr, new_p.ptr, err.ptr, None)
+        # kept slots behind the budget: three quarters of them by chance
+        moved = B * layers * NKV * ((length - budget) * budget // length * 1024 + 8 * (length + budget))
+    flush, ev, ms = DeviceArray((256 << 20,), np.uint8), Events(), 0.0
+    for r in range(warmup + reps):
+        flush.fill_bytes(r & 0xFF)
+        ev.record_start(None)
+        run()
+        ev.record_end(None)
+        ms += ev.elapsed_ms() if r >= warmup else 0.0
+    call("q3_check_error_word", err.ptr, None)
+    us = ms * 1e3 / max(reps, 1)
+    return {"op": name, "batch": B, "length": length, "tokens": tokens, "us": us, "bytes": moved,
+            "gbs": moved / max(us, 1e-9) / 1e3, "l2": "flushed"}
 
 
 class _Graph:
@@ -326,11 +406,23 @@ def main(argv=None) -> int:
     ap.add_argument("--gemv-stream", choices=sorted(GEMV_STREAM_SHAPES), default=None,
                     help="time one projection over all 28 layers per launch")
     ap.add_argument("--reps", type=int, default=20, help="with --gemv-stream: timed launches")
+    ap.add_argument("--cache-op", choices=CACHE_OPS, default=None,
+                    help="time one drafted-token operator (--batch B, --context _ LENGTH, --tokens T)")
+    ap.add_argument("--tokens", type=int, default=8, help="with --cache-op: drafted tokens, or rows of x")
     args = ap.parse_args(argv)
 
     from . import DeviceWeights, Qwen3Decoder, set_device
 
     set_device(args.device)
+    if args.cache_op:
+        r = cache_op(args.cache_op, max(args.batch, 1), args.context[1], args.tokens, args.reps,
+                     0 if args.no_warmup else 3)
+        print(f"  {r['op']} B={r['batch']} length={r['length']} tokens={r['tokens']}: {r['us']:.1f} us, "
+              f"{r['gbs']:.0f} GB/s", flush=True)
+        if args.json:
+            with open(args.json, "w") as f:
+                json.dump(r, f, indent=2)
+        return 0
     dw = DeviceWeights(load_weights(args))
 
     if args.gemv_stream:

@@ -18,7 +18,7 @@ GGUF container (llama.cpp, versions 2 and 3): little-endian magic "GGUF",
 version u32, tensor count u64, metadata count u64, the metadata key/values,
 the tensor infos (name, dims innermost first, ggml type, data offset), then
 the tensor data from the next multiple of general.alignment (default 32).
-ggml types read here: 0 f32, 1 f16, 8 q8_0.
+ggml types read here: 0 f32, 1 f16, 2 q4_0 (raw blocks, for q3_gemv_q4: q4_0 below), 8 q8_0.
 """
 from __future__ import annotations
 
@@ -29,7 +29,8 @@ import numpy as np
 from .weights import DIM, FFN, HD, LAYERS, QBLK, QBYTES, VOCAB, bytes_per_layer
 
 GGUF_MAGIC = 0x46554747
-GGML_F32, GGML_F16, GGML_Q8_0 = 0, 1, 8
+GGML_F32, GGML_F16, GGML_Q4_0, GGML_Q8_0 = 0, 1, 2, 8
+Q4BYTES = 18
 _SCALAR = {0: "<B", 1: "<b", 2: "<H", 3: "<h", 4: "<I", 5: "<i", 6: "<f", 7: "<?", 10: "<Q",
            11: "<q", 12: "<d"}
 
@@ -88,10 +89,11 @@ def read_gguf(path: str):
             nbytes = 4 * n
         elif ttype == GGML_F16:
             nbytes = 2 * n
-        elif ttype == GGML_Q8_0:
+        elif ttype in (GGML_Q4_0, GGML_Q8_0):
             if n % QBLK:
-                raise GGUFError(f"{name}: {n} elements is not a whole number of Q8_0 blocks")
-            nbytes = n // QBLK * QBYTES
+                kind = "Q8_0" if ttype == GGML_Q8_0 else "Q4_0"
+                raise GGUFError(f"{name}: {n} elements is not a whole number of {kind} blocks")
+            nbytes = n // QBLK * (QBYTES if ttype == GGML_Q8_0 else Q4BYTES)
         else:
             tensors[name] = (None, shape, ttype)  # a type the decode path does not read
             continue
@@ -131,6 +133,16 @@ def _q8(tensors, name: str, N: int, K: int) -> np.ndarray:
     raw, shape, ttype = tensors[name]
     if ttype != GGML_Q8_0 or tuple(shape) != (N, K):
         raise GGUFError(f"{name}: {shape} type {ttype}, expected Q8_0 [{N}, {K}]")
+    return np.asarray(raw)
+
+
+def q4_0(tensors, name: str, N: int, K: int) -> np.ndarray:
+    """The raw Q4_0 blocks of a [N, K] matrix, as q3_gemv_q4 reads them."""
+    if name not in tensors:
+        raise GGUFError(f"tensor {name} missing")
+    raw, shape, ttype = tensors[name]
+    if ttype != GGML_Q4_0 or tuple(shape) != (N, K):
+        raise GGUFError(f"{name}: {shape} type {ttype}, expected Q4_0 [{N}, {K}]")
     return np.asarray(raw)
 
 

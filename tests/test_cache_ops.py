@@ -158,3 +158,18 @@ def test_sizes_that_are_not_covered(q3):
     c = Call(q3).with_(**big, new_weight=1 << 40, new_slot_pos=1 << 40)
     assert c.scored() == UNSUPPORTED
     assert c.evict() == UNSUPPORTED
+
+
+def test_gguf_q4_0_blocks(tmp_path, q3):
+    from q3b200 import gguf
+    from test_gguf import _write_gguf
+
+    blocks = quantize(q3, np.random.default_rng(1).standard_normal((8, 256)).astype(np.float32))
+    path = str(tmp_path / "q4.gguf")
+    _write_gguf(path, [("blk.0.attn_q.weight", (8, 256), gguf.GGML_Q4_0, blocks.tobytes()),
+                       ("odd", (3, 11), gguf.GGML_F32, b"\0" * 132)])
+    _, t = gguf.read_gguf(path)
+    assert np.array_equal(gguf.q4_0(t, "blk.0.attn_q.weight", 8, 256), blocks.ravel())
+    for name, N, K in (("none", 8, 256), ("odd", 3, 11), ("blk.0.attn_q.weight", 4, 512)):
+        with pytest.raises(gguf.GGUFError):
+            gguf.q4_0(t, name, N, K)

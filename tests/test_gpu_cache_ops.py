@@ -685,3 +685,11 @@ def test_draft_verify_commit_evict(gpu):
         d["pos"].upload(pos)
     gpu.call("q3_graph_destroy", ex)
     gpu.call("q3_stream_destroy", st)
+
+
+@pytest.mark.parametrize("op", ["q4", "tree", "scored", "evict"])
+def test_benchmark_command(gpu, op, capsys):
+    from q3b200.benchmark import main
+
+    assert main(["--cache-op", op, "--batch", "2", "--context", "0", "500", "--tokens", "6", "--reps", "2"]) == 0
+    assert op in capsys.readouterr().out
