@@ -473,6 +473,8 @@ int q3_batch_trace_kernels(q3_batch* m, int64_t steps, long long* out, int32_t* 
  * allocating or synchronising, take no workspace, can be captured into
  * graphs and run concurrently with one another on different buffers.
  *
+ * Pointers are aligned to their element types unless more is said.
+ *
  * Device-side checks: counts, lengths, positions and trees are DEVICE data.
  * A sequence whose values are out of range is left as it was (its outputs and
  * cache are not written) and a code goes into the device word *err if that is

@@ -1064,6 +1064,7 @@ __global__ void __launch_bounds__(128) k_tree_commit(const CommitArgs a) {
   const int n = a.n_accepted[b];
   const int64_t len = a.len[b];
   bool bad = n < 0 || n > a.A || len < 0 || len > a.S - n;
+  if (a.pos != nullptr) bad |= a.pos[b] < 0 || a.pos[b] > INT32_MAX - kTreeMaxTokens;  // slot_pos holds 32 bits
   const int32_t* acc = a.accepted + (int64_t)b * a.A;
   if (!bad) {
     for (int i = lane; i < n; i += 32) {

@@ -138,6 +138,21 @@ def test_argument_refusals(q3, op, change):
     assert getattr(Call(q3).with_(**change), op)() == INVALID
 
 
+ALIGNED = {"tree": {2: ("q_norm", "k_norm"), 4: ("cos", "sin", "parents", "n", "err"), 8: ("qkv", "out", "len", "pos")},
+           "scored": {2: ("q_norm", "k_norm"), 4: ("cos", "sin", "weight", "new_weight", "slot_pos", "err"),
+                      8: ("qkv", "out", "len", "pos")},
+           "commit": {4: ("accepted", "n", "weight", "slot_pos", "err"), 8: ("len", "new_len", "pos")},
+           "evict": {4: ("weight", "slot_pos", "new_weight", "new_slot_pos", "err"), 8: ("len", "new_len", "pos")}}
+
+
+@pytest.mark.parametrize("op,name,size", [(op, n, s) for op, a in ALIGNED.items() for s, ns in a.items() for n in ns])
+def test_misaligned_arrays(q3, op, name, size):
+    c = Call(q3)
+    c.a[name] = (c.a[name] or c.p + 32768) + size // 2
+    assert getattr(c, op)() == INVALID
+    assert b"aligned" in q3.lib().q3_last_error()
+
+
 def test_overlapping_arrays(q3):
     c = Call(q3)
     assert c.with_(new_len=c.p + 8).commit() == INVALID

@@ -36,7 +36,9 @@ def gemv_tolerance(blocks, x):
 
 @pytest.mark.parametrize("N,K,R", [(1, 256, 1), (15, 256, 2), (16, 512, 1), (17, 768, 3), (100, 1024, 7), (2048, 1024, 1),
                                    (1000, 1280, 8), (6007, 1280, 5), (33, 2048, 9), (48, 2304, 16), (20, 16384, 1),
-                                   (20, 16384, 16), (4099, 256, 12), (40000, 512, 8), (50021, 1024, 4)])
+                                   (20, 16384, 16), (4099, 256, 12), (40000, 512, 8), (50021, 1024, 4),
+                                   (20000, 768, 16), (12000, 2048, 3), (13001, 1280, 9), (10007, 256, 1),
+                                   (9990, 4096, 2)])
 def test_gemv_q4(gpu, N, K, R):
     rng = np.random.default_rng(N + K + R)
     blocks, x = q4_blocks(rng, N, K), rng.standard_normal((R, K)).astype(np.float16)
@@ -412,6 +414,17 @@ def test_tree_commit_bad_values(gpu):
     w = c.k.copy()
     c.view(w)[0, :, :, 10:13] = c.view(c.k)[0, :, :, [11, 13, 15]].transpose(1, 2, 0, 3)
     assert np.array_equal(bits(c.download()[0]), bits(w))
+
+
+@pytest.mark.parametrize("pos", [-1, 1 << 31])
+def test_tree_commit_bad_position(gpu, pos):
+    c = Cache(np.random.default_rng(3), 1, 1, 90).upload(gpu)
+    w, sp = np.ones((1, 1, 8, 90), np.float32), np.full((1, 1, 8, 90), 5, np.int32)
+    given = [up(gpu, x) for x in (np.array([pos]), w, sp)]
+    new_len, err = commit(gpu, c, 0, 1, np.array([[1, 2]], np.int32), np.array([2], np.int32), np.array([10]), given)
+    assert err == BAD_TREE and new_len[0] == 10
+    assert np.array_equal(given[1].download(), w) and np.array_equal(given[2].download(), sp)
+    assert np.array_equal(bits(c.download()[0]), bits(c.k))
 
 
 # ------------------------------------------------------------------------ scored
