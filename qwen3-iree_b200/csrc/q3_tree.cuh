@@ -124,13 +124,13 @@ struct TreeCta {
   int parent;                       // of token `tid`
 };
 
-// Reads and checks the sequence's values; false: nothing to do (the same in all CTAs of a cluster).
 __device__ __forceinline__ void tree_place(TreeCta& c) {
   c.C = gridDim.x, c.rank = blockIdx.x, c.h = blockIdx.y, c.b = blockIdx.z;
   c.fresh = c.rank == c.C - 1;
   c.tid = threadIdx.x, c.lane = c.tid & 31;
   c.warp = __shfl_sync(0xffffffffu, c.tid >> 5, 0);  // uniform for the compiler too
 }
+// Reads and checks the sequence's values; false: nothing to do (the same in all CTAs of a cluster).
 template <bool SCORED>
 __device__ __forceinline__ bool tree_begin(const TreeArgs& a, TreeCta& c) {
   c.n = SCORED ? 1 : (a.n_tokens ? a.n_tokens[c.b] : a.T);

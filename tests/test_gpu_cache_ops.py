@@ -347,6 +347,24 @@ def test_tree_attention_is_deterministic_and_captured(gpu):
     gpu.call("q3_stream_destroy", s)
 
 
+def test_smallest_cache(gpu):
+    """One slot, one head, one sequence: the strides of all dimensions but the row's are unused."""
+    t = Scored(gpu, 50, [0], S=1, q_heads=1, kv_heads=1)
+    t.upload()
+    t.c.kv = gpu.KVCache(t.c.dk.ptr, t.c.dv.ptr, 0, 0, 0, 0, 1, 1, 1, 1)
+    t.call().check()
+    t = Tree(gpu, 51, 1, [0], S=1, q_heads=1, kv_heads=1)
+    t.upload()
+    t.c.kv = gpu.KVCache(t.c.dk.ptr, t.c.dv.ptr, 0, 0, 0, 0, 1, 1, 1, 1)
+    t.call().check()
+    c = Cache(np.random.default_rng(1), 1, 1, 1, 1, 1).upload(gpu)
+    c.kv = gpu.KVCache(c.dk.ptr, c.dv.ptr, 0, 0, 0, 0, 1, 1, 1, 1)
+    new_len, err = commit(gpu, c, 0, 1, np.zeros((1, 1), np.int32), np.array([1], np.int32), np.array([0]))
+    assert err == 0 and new_len[0] == 1
+    w = np.ones((1, 1, 1, 1), np.float32)
+    assert run_evict(gpu, c, 0, 1, w, w.astype(np.int32), np.array([1]), np.array([1]), 1, 0) == 0
+
+
 def test_two_streams(gpu):
     """Calls on different buffers at the same time."""
     ts = [Tree(gpu, 20 + i, T, [n], S=3000).upload() for i, (T, n) in enumerate([(3, 2900), (64, 2500), (20, 1000)])]
