@@ -13,9 +13,8 @@
 // Selection: keys are the weights' bits in an order-preserving form, above them all the newest.  A
 // histogram of their top 11 bits gives the bin of the M-th largest; its keys, some tens, are ranked by
 // counting, or by two more histograms where there are many.  Ballots then give each slot's fate and its
-// rank in slot order.  28 layers of 1024 slots, 512 kept: selection 8 us, moves 8
-// (at the copy rate).  Small CTAs, many to
-// an SM, so that some select while others move.
+// rank in slot order.  28 layers of 1024 slots, 512 kept: selection 8 us, moves 8 (at the copy rate).
+// Small CTAs, many to an SM, so that some select while others move.
 #pragma once
 
 #include "q3_common.cuh"
