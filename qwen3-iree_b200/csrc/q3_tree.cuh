@@ -905,10 +905,11 @@ __global__ void __launch_bounds__(kTreeTcThreads, 2) k_tree_tc(const __grid_cons
     int s = 0, sp = 0;            // slots of K of tile j and of V of tile j - 1
     uint32_t ph = 0, php = 0;     // their phases
     for (int j = 0; j <= c.tiles; ++j) {
+      // the weights of tile j - 2 share the S buffer; and o_done may have one phase open at most, in the
+      // last round too: a wait by parity takes a phase two behind for the one it is for
+      if (j >= 2) ok &= mbar_wait_own(&sm.o_done, j & 1, a.err, kErrTimeoutFull);
       if (j < c.tiles) {
         ok &= mbar_wait_own(&sm.k_full[s], ph, a.err, kErrTimeoutFull);
-        // the weights of tile j - 2 share this S buffer
-        if (j >= 2) ok &= mbar_wait_own(&sm.o_done, j & 1, a.err, kErrTimeoutFull);
         if (!__all_sync(0xffffffffu, ok)) break;
         tc_fence_after();
         if (leader) {
