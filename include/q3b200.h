@@ -519,7 +519,9 @@ typedef struct q3_kv_cache {
  *             len < pos
  *   out:      f16 [B][T][q_heads * 128], 8-byte aligned like qkv
  * 1 <= T <= 64 and T * q_heads / kv_heads <= 128.  rope tables f32
- * [rope_rows, 64].  Tolerance-level parity; deterministic. */
+ * [rope_rows, 64].  Tolerance-level parity; deterministic.  Softmax weights are
+ * rounded to f16 for the product with V (2^-11 of a weight down to 2^-23 of the
+ * row's largest, 2^-34 of that below); maxima and sums are f32. */
 int q3_tree_attention(const void* qkv, const void* q_norm, const void* k_norm,
                       const float* rope_cos, const float* rope_sin, int64_t rope_rows,
                       const q3_kv_cache* cache, int layer, int B, int T, const int32_t* parents,

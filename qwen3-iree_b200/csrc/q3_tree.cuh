@@ -37,6 +37,14 @@ constexpr int kTreeMaxDepth = 6;                          // tiles a ring holds
 constexpr int kTreeSmallRows = 16;                        // rows of k_tree_attn
 constexpr int kTreeRows = 128;                            // most rows of k_tree_tc
 constexpr float kTreeLog2Scale = kAttnScale * 1.44269504088896341f;  // scores in powers of two
+// The softmax weights go to P V as f16, relative to a reference that puts the largest near 2^15, the top
+// of that type: then a weight down to 2^-29 of the largest keeps half a step of 2^-11 of itself, and a
+// smaller one is off by at most 2^-40 of the largest.  (With the largest at 1 these were 2^-14 and 2^-25:
+// over a cache whose first slots draw nearly everything, as they do in trained models, the others' share
+// lost digits or vanished.)  Where an output is rescaled late, by kTreeLazy powers of two at most, the
+// reference starts that much lower: 2^-23 and 2^-34 (64 tokens over 32749 slots: 48.2 us with 8, 48.4
+// with 6, 50.1 with 4).  Sums share the reference, so quotients do not change.
+constexpr float kTreeTop = 15.0f, kTreeLazy = 6.0f;
 
 struct TreeArgs {
   CUtensorMap km, vm;   // the layer's K and V: {dim, slot, head, sequence}, boxes of 64 dims x 64 slots
@@ -80,6 +88,10 @@ __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+// The reference that puts a score of `top` at 2^exponent.  Steps of f32 above 2^20 are too coarse for it.
+__device__ __forceinline__ float tree_ref(float top, float exponent) {
+  return fabsf(top) < 1048576.0f ? __fsub_rn(top, exponent) : top;
 }
 __device__ __forceinline__ uint32_t pack_h2(float lo, float hi) {
   const __half2 h = __floats2half2_rn(lo, hi);
@@ -566,7 +578,7 @@ __global__ void __launch_bounds__(kTreeThreads, 3)
           float mx = fmaxf(fmaxf(s[0][2 * e], s[0][2 * e + 1]), fmaxf(s[1][2 * e], s[1][2 * e + 1]));
           mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
           mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-          const float mn = fmaxf(m[e], __fmul_rn(mx, kTreeLog2Scale));
+          const float mn = fmaxf(m[e], tree_ref(__fmul_rn(mx, kTreeLog2Scale), kTreeTop));
           const float mu = mn == -INFINITY ? 0.0f : mn;  // a row that sees no key yet
           const float al = ex2(__fsub_rn(m[e], mu));
           m[e] = mn;
@@ -772,8 +784,8 @@ static_assert(tree_tc_bytes<128>() <= 233472 / 2 - 1024 && tree_tc_bytes<64>() <
 //                 when the weights of tile j - 1 are written, O += P V (4 of 128 x 128 x 16); so S(j)
 //                 runs during the softmax of tile j - 1
 //   softmax warps thread r holds row r: one TMEM lane, no shuffles.  O stays in TMEM; it is rescaled
-//                 only when a row's maximum has grown by more than 2^8 over its reference (weights
-//                 relative to it stay below 2^8; sum and output share it, so the quotient is the same)
+//                 only when a row's maximum has grown by more than kTreeLazy since the last time (each
+//                 time costs a pass over its 128 columns; sum and output share the reference)
 // Measured: 64 tokens over 32749 slots 48 us (2.8 TB/s, 355 TFLOP/s), of which 13 are preparation and
 // merge and a tile takes a CTA 0.8; 17 tokens x 16 sequences to 4001 40 us (3.7 TB/s).
 template <int ROWS>
@@ -856,7 +868,7 @@ __global__ void __launch_bounds__(kTreeTcThreads, 2) k_tree_tc(const __grid_cons
   tc_fence_after();
   const uint32_t tmem = sm.tmem;
   const bool live = warp * 32 < c.R;  // softmax warps of padding rows have nothing to do
-  float m = -INFINITY, l = 0.0f;
+  float m = -INFINITY, l = 0.0f, limit = -INFINITY;  // reference, sum, the score from which it is moved
 
   if (warp == 4) {
     // K runs KD - VD tiles ahead of V, whose slots are freed later
@@ -970,8 +982,9 @@ __global__ void __launch_bounds__(kTreeTcThreads, 2) k_tree_tc(const __grid_cons
 #pragma unroll
       for (int i = 0; i < 64; ++i) mx[i & 3] = fmaxf(mx[i & 3], __uint_as_float(u[i]));
       const float top = __fmul_rn(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])), kTreeLog2Scale);
-      const bool grow = row < c.R && top > __fadd_rn(m, 8.0f);  // from -inf: the first key that counts
-      const float mn = grow ? top : m;
+      const bool grow = row < c.R && top > limit;  // from -inf: the first key that counts
+      const float mn = grow ? tree_ref(top, kTreeTop - kTreeLazy) : m;
+      if (grow) limit = __fadd_rn(top, kTreeLazy);
       const float mu = mn == -INFINITY ? 0.0f : mn;
       if (j > 0 && __any_sync(0xffffffffu, grow)) {
         ok &= mbar_wait_own(&sm.o_done, (j - 1) & 1, a.err, kErrTimeoutFull);
