@@ -103,8 +103,8 @@ __global__ void __launch_bounds__(kEvictThreads, 6) k_cache_evict(const EvictArg
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int b = blockIdx.z, layer = blockIdx.y / a.kv_heads, h = blockIdx.y - layer * a.kv_heads;
   const int64_t len64 = a.len[b];
-  const int64_t newest = a.pos[b] - a.recent;
-  const bool bad = len64 < 0 || len64 > a.S;
+  const int64_t pos = a.pos[b], newest = pos - a.recent;
+  const bool bad = len64 < 0 || len64 > a.S || pos < 0;
   const int len = bad ? 0 : (int)len64;
   const int M = (int)a.budget, held = len < M ? len : M;
   if (blockIdx.x == 0 && blockIdx.y == 0 && tid == 0) {
