@@ -532,7 +532,7 @@ int q3_tree_attention(const void* qkv, const void* q_norm, const void* k_norm,
  * n = n_accepted[b] (strictly ascending indices < 64 of drafted tokens), move
  * from slots len[b] + accepted[b][i] to len[b] + i, in layers
  * layer0..layer0+n_layers-1; new_len[b] = len[b] + n.  accepted: DEVICE int32
- * [B][A], A <= 64; new_len lies apart from len.  A bad path moves nothing and
+ * [B][A], A <= 64; new_len lies apart from len and pos.  A bad path moves nothing and
  * gives new_len[b] = len[b].  Where the cache is evicted from (below), pos,
  * weight and slot_pos are given (all three or none): the accepted slots start
  * with weight 0 and hold positions pos[b] + i, the path's depths. */
@@ -563,7 +563,8 @@ int q3_decode_attention_scored(const void* qkv, const void* q_norm, const void* 
  * depend on slot order, so kept slots below the budget stay where they are, and
  * those behind it move, in order, into the holes: K/V in place, weights and
  * positions from weight / slot_pos to new_weight / new_slot_pos (apart from
- * them).  new_len[b] = min(len[b], budget); nothing behind it is written.
+ * them).  new_len[b] = min(len[b], budget) (apart from len and pos); nothing
+ * behind it is written.
  * pos: the sequence's next position.  recent <= budget; slots <= 524288. */
 int q3_cache_evict(const q3_kv_cache* cache, int layer0, int n_layers, int B, int64_t budget,
                    int64_t recent, const int64_t* len, const int64_t* pos, const float* weight,
