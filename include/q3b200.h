@@ -489,7 +489,9 @@ int q3_quantize_q4_0(const float* w, int64_t n, uint8_t* out);
 
 /* Q4_0 fused dequant + GEMV for R rows: y[R][N] = x[R][K] . W[N][K]^T, f32
  * sums (tensor cores), f16 out, tolerance-level parity.  1 <= R <= 16, N >= 1,
- * K multiple of 256, K <= 16384; w ([N][K/32] blocks) and x 16-byte aligned. */
+ * K multiple of 256, K <= 16384; w ([N][K/32] blocks) and x 16-byte aligned.
+ * Where a wait inside the kernel gives up (about a second: a device in trouble)
+ * the outputs that it has no sum for are NaN. */
 int q3_gemv_q4(const void* w, const void* x, void* y, int N, int K, int R, void* stream);
 
 /* A KV cache: f16 rows of 128, element (sequence b, layer l, slot s, kv head h)

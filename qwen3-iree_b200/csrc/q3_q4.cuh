@@ -288,11 +288,12 @@ __global__ void __launch_bounds__(kQ4StreamMaxGroups * kQ4StreamSplit * 32, 1) k
   const int at = (g >> lg) * (ub + 16) + (g & (s.copy_rows - 1)) * rb;
   const int at8 = (g8 >> lg) * (ub + 16) + (g8 & (s.copy_rows - 1)) * rb;
   const int np = a.K / 64 / KW, p0 = part * np;  // even: K is a multiple of 256
-  int st = 0;
+  int st = 0, tile = t0;
   uint32_t ph = 0;
   bool ok = true;
-  for (int tile = t0; tile < t1; tile += groups) {
-    ok &= mbar_wait_own(&full[grp][st], ph, nullptr, kErrTimeoutFull);
+  for (; tile < t1; tile += groups) {
+    ok = mbar_wait_own(&full[grp][st], ph, nullptr, kErrTimeoutFull);
+    if (!__all_sync(0xffffffffu, ok)) break;
     uint32_t w0 = rg + st * s.stage + at + 36 * p0, w1 = rg + st * s.stage + at8 + 36 * p0;
     uint32_t xb = smem_u32(xs) + lane * 16 + p0 * (NT * 1024);
     float acc[NT][4] = {};
@@ -312,14 +313,15 @@ __global__ void __launch_bounds__(kQ4StreamMaxGroups * kQ4StreamSplit * 32, 1) k
       __syncwarp();
       if (lane == 0) mbar_arrive(&done[grp][st]);
     } else {
-      ok &= mbar_wait_own(&done[grp][st], ph, nullptr, kErrTimeoutFull);
+      ok = mbar_wait_own(&done[grp][st], ph, nullptr, kErrTimeoutFull);
+      if (!__all_sync(0xffffffffu, ok)) break;
 #pragma unroll
       for (int k = 0; k < KW - 1; ++k)
 #pragma unroll
         for (int i = 0; i < 4 * NT; ++i)
           acc[i >> 2][i & 3] = __fadd_rn(acc[i >> 2][i & 3], at_sums[(k * 4 * NT + i) * 32]);
       __syncwarp();  // all are done with the stage and the sums have been read
-      if (ok && tile + kQ4StreamStages * groups < t1) issue(tile + kQ4StreamStages * groups, st);
+      if (tile + kQ4StreamStages * groups < t1) issue(tile + kQ4StreamStages * groups, st);
       const int row = tile * 16 + g;
 #pragma unroll
       for (int i = 0; i < 4 * NT; ++i) {
@@ -328,6 +330,18 @@ __global__ void __launch_bounds__(kQ4StreamMaxGroups * kQ4StreamSplit * 32, 1) k
       }
     }
     if (++st == kQ4StreamStages) st = 0, ph ^= 1;
+  }
+  // a wait gave up: there is no error word here, so the rows without a sum become NaN
+  if (part == 0 && tile < t1) {
+    for (int i = 0; i < kQ4StreamStages && tile + i * groups < t1; ++i) {  // copies under way land first
+      mbar_wait_own(&full[grp][st], ph, nullptr, kErrTimeoutFull);
+      if (++st == kQ4StreamStages) st = 0, ph ^= 1;
+    }
+    for (; tile < t1; tile += groups)
+      for (int i = lane; i < 16 * a.R; i += 32) {
+        const int w = tile * 16 + (i & 15);
+        if (w < a.N) a.y[(int64_t)(i >> 4) * a.N + w] = 0x7fff;
+      }
   }
 }
 

@@ -3,8 +3,8 @@ against the plain 64-bit forms (cache_reference)."""
 import numpy as np
 import pytest
 
-from cache_reference import HD, attend, norm_rope, paths
-from test_gpu_cache_ops import Scored, Tree, bits
+from cache_reference import HD, attend, norm_rope, paths, q4_blocks, q4_dequant
+from test_gpu_cache_ops import Scored, Tree, bits, gemv
 
 pytestmark = pytest.mark.gpu
 
@@ -130,3 +130,22 @@ def test_tree_huge_scores(gpu, T, gamma):
     t.gq[:] = gamma
     t.c.view(t.c.k)[0, 0, :, 40] = 60000
     assert np.isfinite(t.upload().call().check()).all()
+
+
+# ------------------------------------------------------------------------- 4-bit GEMV
+@pytest.mark.parametrize("N,K,R", [(151936, 256, 1), (151936, 256, 16), (151936, 1024, 8), (151936, 1024, 16),
+                                   (90001, 1280, 3), (60007, 2048, 8), (151935, 512, 9)])
+def test_gemv_q4_of_many_tiles(gpu, N, K, R):
+    """Every ring stage of the streaming kernel is filled several times; and the same bits again."""
+    rng = np.random.default_rng(N + K + R)
+    blocks, x = q4_blocks(rng, N, K), rng.standard_normal((R, K)).astype(np.float16)
+    got = gemv(gpu, blocks, x)
+    xd = x.astype(np.float64)
+    for n in range(0, N, 8192):
+        w = q4_dequant(blocks[n:n + 8192])
+        y = xd @ w.T
+        # 32 exact products of a block summed in f32 by two MMAs, a chain of K / 64 blocks a warp, the
+        # two warps' sums: each step off by up to 2^-23 of the sum of magnitudes; one rounding to f16
+        tol = (34 + K / 64 + 2) * 2.0 ** -23 * (np.abs(xd) @ np.abs(w).T) + 2.0 ** -11 * np.abs(y) + 2.0 ** -25
+        assert (np.abs(got[:, n:n + 8192] - y) <= tol).all(), n
+    assert np.array_equal(bits(gemv(gpu, blocks, x)), bits(got))
