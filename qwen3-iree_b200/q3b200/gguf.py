@@ -89,16 +89,20 @@ def read_gguf(path: str):
             nbytes = 4 * n
         elif ttype == GGML_F16:
             nbytes = 2 * n
-        elif ttype in (GGML_Q4_0, GGML_Q8_0):
+        elif ttype == GGML_Q8_0:
             if n % QBLK:
-                kind = "Q8_0" if ttype == GGML_Q8_0 else "Q4_0"
-                raise GGUFError(f"{name}: {n} elements is not a whole number of {kind} blocks")
-            nbytes = n // QBLK * (QBYTES if ttype == GGML_Q8_0 else Q4BYTES)
+                raise GGUFError(f"{name}: {n} elements is not a whole number of Q8_0 blocks")
+            nbytes = n // QBLK * QBYTES
+        elif ttype == GGML_Q4_0 and n % QBLK == 0:
+            nbytes = n // QBLK * Q4BYTES
         else:
-            tensors[name] = (None, shape, ttype)  # a type the decode path does not read
+            tensors[name] = (None, shape, ttype)  # not read by the decode path
             continue
         start = data0 + toff
         if start + nbytes > len(buf):
+            if ttype == GGML_Q4_0:  # the decode path does not read these either
+                tensors[name] = (None, shape, ttype)
+                continue
             raise GGUFError(f"{name}: data runs past the end of the file")
         tensors[name] = (buf[start:start + nbytes], shape, ttype)
     return meta, tensors
@@ -143,6 +147,8 @@ def q4_0(tensors, name: str, N: int, K: int) -> np.ndarray:
     raw, shape, ttype = tensors[name]
     if ttype != GGML_Q4_0 or tuple(shape) != (N, K):
         raise GGUFError(f"{name}: {shape} type {ttype}, expected Q4_0 [{N}, {K}]")
+    if raw is None:
+        raise GGUFError(f"{name}: not whole Q4_0 blocks, or cut short")
     return np.asarray(raw)
 
 
