@@ -473,7 +473,9 @@ int q3_batch_trace_kernels(q3_batch* m, int64_t steps, long long* out, int32_t* 
  * allocating or synchronising, take no workspace, can be captured into
  * graphs and run concurrently with one another on different buffers.
  *
- * Pointers are aligned to their element types unless more is said.
+ * Pointers are aligned to their element types unless more is said.  What a call
+ * writes lies apart from what it reads and from what else it writes, unless
+ * the call says that it works in place.
  *
  * Device-side checks: counts, lengths, positions and trees are DEVICE data.
  * A sequence whose values are out of range is left as it was (its outputs and
