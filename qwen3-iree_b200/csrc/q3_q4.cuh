@@ -32,10 +32,8 @@ struct Q4GemvArgs {
   int pitch;          // bytes between weight rows in shared memory
 };
 
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool take) {
-  const int n = take ? 16 : 0;  // 0: the 16 bytes are filled with zeros, src is not read
-  asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n)
-               : "memory");
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -160,7 +158,7 @@ __global__ void __launch_bounds__(kQ4Warps * 32) k_gemv_q4(const Q4GemvArgs a) {
   const uint8_t* src = a.w + (int64_t)row0 * rb;
   for (int i = threadIdx.x; i < nrow * chunks; i += blockDim.x) {
     const int r = i / chunks;
-    cp_async16(smem_u32(ws) + r * a.pitch + (i - r * chunks) * 16, src + (int64_t)i * 16, true);
+    cp_async16(smem_u32(ws) + r * a.pitch + (i - r * chunks) * 16, src + (int64_t)i * 16);
   }
   cp_commit();
   const int npair = a.K / 64;

@@ -33,9 +33,8 @@ constexpr int kTreeHalf = kTreeTile * kHD * 2;            // a stage: K, then V
 constexpr int kTreeStageBytes = 2 * kTreeHalf;
 constexpr int kTreeOPitch = kHD + 4;                      // floats between partial output rows
 constexpr int kTreeMaxCluster = 16;
-constexpr int kTreeMaxDepth = 6;                          // tiles a ring holds
+constexpr int kTreeMaxDepth = 3;                          // tiles a ring of k_tree_attn holds, two or three
 constexpr int kTreeSmallRows = 16;                        // rows of k_tree_attn
-constexpr int kTreeRows = 128;                            // most rows of k_tree_tc
 constexpr float kTreeLog2Scale = kAttnScale * 1.44269504088896341f;  // scores in powers of two
 // The softmax weights go to P V as f16, relative to a reference that puts the largest near 2^15, the top
 // of that type: then a weight down to 2^-29 of the largest keeps half a step of 2^-11 of itself, and a
