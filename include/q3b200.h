@@ -480,8 +480,8 @@ int q3_batch_trace_kernels(q3_batch* m, int64_t steps, long long* out, int32_t* 
  * Device-side checks: counts, lengths, positions and trees are DEVICE data.
  * A sequence whose values are out of range is left as it was (its outputs and
  * cache are not written) and a code goes into the device word *err if that is
- * 0 (5: length, count or position; 6: tree or path); err may be NULL; read it
- * with q3_check_error_word. */
+ * 0 (5: length, count or position; 6: tree or path, and all that
+ * q3_tree_commit refuses); err may be NULL; read it with q3_check_error_word. */
 
 /* Q4_0 quantizer on host memory (n multiple of 32; out: n/32*18 bytes): blocks
  * of 32 as GGUF holds them, [f16 d | 16 bytes], byte j with value j in its low
@@ -524,8 +524,8 @@ typedef struct q3_kv_cache {
  *   out:      f16 [B][T][q_heads * 128], 8-byte aligned like qkv
  * 1 <= T <= 64 and T * q_heads / kv_heads <= 128.  rope tables f32
  * [rope_rows, 64].  Tolerance-level parity; deterministic.  Softmax weights are
- * rounded to f16 for the product with V (2^-11 of a weight down to 2^-23 of the
- * row's largest, 2^-34 of that below); maxima and sums are f32. */
+ * rounded to f16 for the product with V: each by at most 2^-11 of itself, or
+ * 2^-34 of the row's largest; maxima and sums are f32. */
 int q3_tree_attention(const void* qkv, const void* q_norm, const void* k_norm,
                       const float* rope_cos, const float* rope_sin, int64_t rope_rows,
                       const q3_kv_cache* cache, int layer, int B, int T, const int32_t* parents,
@@ -536,8 +536,9 @@ int q3_tree_attention(const void* qkv, const void* q_norm, const void* k_norm,
  * n = n_accepted[b] (strictly ascending indices < 64 of drafted tokens), move
  * from slots len[b] + accepted[b][i] to len[b] + i, in layers
  * layer0..layer0+n_layers-1; new_len[b] = len[b] + n.  accepted: DEVICE int32
- * [B][A], A <= 64; new_len lies apart from len and pos.  A bad path moves nothing and
- * gives new_len[b] = len[b].  Where the cache is evicted from (below), pos,
+ * [B][A], A <= 64; new_len lies apart from len and pos.  A path that is
+ * bad or does not fit (its count, the length, pos) moves nothing and gives
+ * new_len[b] = len[b] and code 6.  Where the cache is evicted from (below), pos,
  * weight and slot_pos are given (all three or none): the accepted slots start
  * with weight 0 and hold positions pos[b] + i, the path's depths. */
 int q3_tree_commit(const q3_kv_cache* cache, int layer0, int n_layers, int B, int A,

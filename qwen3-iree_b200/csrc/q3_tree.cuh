@@ -785,8 +785,10 @@ static_assert(tree_tc_bytes<128>() <= 233472 / 2 - 1024 && tree_tc_bytes<64>() <
 //   softmax warps thread r holds row r: one TMEM lane, no shuffles.  O stays in TMEM; it is rescaled
 //                 only when a row's maximum has grown by more than kTreeLazy since the last time (each
 //                 time costs a pass over its 128 columns; sum and output share the reference)
-// Measured: 64 tokens over 32749 slots 48 us (2.8 TB/s, 355 TFLOP/s), of which 13 are preparation and
-// merge and a tile takes a CTA 0.8; 17 tokens x 16 sequences to 4001 40 us (3.7 TB/s).
+// Measured: 64 tokens over 32749 slots 48.4 us (2.8 TB/s, 355 TFLOP/s).  128 CTAs on 114 SMs: preparation
+// 7 to 9, then 33 tiles in 26 on an SM of its own (0.78 a tile) and in 31 beside another CTA (0.94), which
+// 28 of them are and all wait for; merge and output 9 to 10 (time stamps, which add about 4 in all).
+// 17 tokens x 16 sequences to 4001: 39.7 us (3.7 TB/s).
 template <int ROWS>
 __global__ void __launch_bounds__(kTreeTcThreads, 2) k_tree_tc(const __grid_constant__ TreeArgs a) {
   using L = TreeTc<ROWS>;
