@@ -144,7 +144,7 @@ __device__ __forceinline__ void q4_pair(uint32_t a, uint32_t a8, uint32_t at, ui
 constexpr int kQ4PartPitch = 20;  // floats between x rows of a warp's partial sums: no bank conflict
 
 // One CTA per 16 weight rows; its 8 warps take the row's pairs of blocks in turn.  Bound by the launch
-// and one memory round trip: 2048 x 1024, one row, 2.6 us; 6007 x 1280, three rows, 3.8 us.  The rows arrive
+// and one memory round trip: 2048 x 1024, one row, 2.6 us; 6007 x 1280, three rows, 3.7 us.  The rows arrive
 // by cp.async while the warps load their x.
 template <int NT>
 __global__ void __launch_bounds__(kQ4Warps * 32) k_gemv_q4(const Q4GemvArgs a) {
@@ -203,8 +203,8 @@ __global__ void __launch_bounds__(kQ4Warps * 32) k_gemv_q4(const Q4GemvArgs a) {
 // A bulk copy takes the SM's copy engine about 30 cycles whatever its size (151936 x 1024 in copies of
 // 288 bytes: 37 us, of 1152: 25), so a copy is as many rows as keep the fragment loads free of bank
 // conflicts: rows are 36 K/256 words apart, so 8 / gcd(8, K/256) neighbouring rows fall into different
-// banks, and 16 bytes between the copies shift the next ones.  151936 x 1024, 8 rows: 24.6 us, 3.7 TB/s;
-// the copies alone take 18, the arithmetic alone 19.
+// banks, and 16 bytes between the copies shift the next ones.  151936 x 1024, 8 rows: 24.4 us, 3.6
+// TB/s (16 rows 35); the copies alone take 18, the arithmetic alone 19.
 constexpr int kQ4StreamSplit = 2;       // KW
 constexpr int kQ4StreamMaxGroups = 10;
 constexpr int kQ4StreamStages = 2;

@@ -439,7 +439,7 @@ __device__ __forceinline__ void tree_output(const TreeArgs& a, const TreeCta& c,
 // state of its own, so a tile costs it 16 + 16 MMAs and one pass over its K and V fragments.  Bound by
 // the copies where there is work for all SMs (scored, four sequences of 8000: 28.8 us, 4.6 TB/s; 32 of
 // 2000: 50 us, 5.3 TB/s), by a chain of round trips (lengths, rows, tiles, merge) where there is little
-// (8 tokens over 500 slots: 9.1 us).
+// (8 tokens over 500 slots: 9.2 us).
 struct TreeSmallSmem {  // behind the ring
   uint8_t q[kTreeSmallRows * 256];
   float2 mlw[4][kTreeSmallRows];  // the warps' (max, sum)
